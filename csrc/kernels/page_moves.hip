@@ -1,0 +1,254 @@
+// Pages of the K/V cache that change their place: copies (a sequence forks, a thread moves) and the compaction of sequences
+// whose tokens leave.  Caches are [layers][pages][kv heads][PAGE][row], K and V, with strides between layers, pages and heads;
+// a token's row of a head is row_bytes contiguous bytes, a page of a head PAGE rows.
+#include "common.h"
+
+namespace {
+
+constexpr int PAGE = 64;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+struct Cache {   // strides in bytes
+  char* p;
+  long layer, page, head;
+};
+
+// ---- copies ----
+// The pairs travel in the launch's own arguments: no copy to the device and no memory to keep until the launch has run.
+constexpr int PAIRS = 256;
+struct Pairs {
+  int src[PAIRS], dst[PAIRS];
+  uint8_t tokens[PAIRS];
+};
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(Cache k, Cache v, Pairs pairs, int heads, int layers, int row_bytes) {
+  const int h = blockIdx.x % heads, layer = blockIdx.x / heads % layers, i = blockIdx.x / heads / layers;
+  const Cache c = blockIdx.y ? v : k;
+  const int n = pairs.tokens[i] * row_bytes / 16;
+  const long at = layer * c.layer + h * c.head;
+  const u32x4* from = (const u32x4*)(c.p + at + pairs.src[i] * c.page);
+  u32x4* to = (u32x4*)(c.p + at + pairs.dst[i] * c.page);
+  for (int j = threadIdx.x; j < n; j += 256) to[j] = from[j];
+}
+
+// ---- compaction ----
+struct Sequences {
+  const int *tables, *to, *lens;      // tables, to: [n][width]; to null: in place
+  const uint8_t* keep;                // [n][places], rows keep_stride apart
+  int width, table_stride, to_stride, places, num_pages;
+  long keep_stride;
+  int* new_lens;
+};
+
+__device__ __forceinline__ int length_of(const Sequences& s, int seq) {
+  return max(0, min(s.lens[seq], min(s.places, s.width * PAGE)));
+}
+
+// A thread holds 16 bytes of each half of a token's row (numbers d and d + 64 of a rotated key meet in one thread), so a
+// token takes TPT = row_bytes / 32 threads.
+struct Row {
+  u32x4 lo, hi;
+};
+
+__device__ __forceinline__ Row load_row(const char* p, int half) { return {*(const u32x4*)p, *(const u32x4*)(p + half)}; }
+__device__ __forceinline__ void store_row(char* p, int half, const Row& r) {
+  *(u32x4*)p = r.lo;
+  *(u32x4*)(p + half) = r.hi;
+}
+
+// Key numbers i and i + 64, rotated for place `from`, turned on to place `to`: by the angle between the two, whose cosine and
+// sine come from the table's of both places in fp32; one rounding to bf16 at the end.
+struct Turn {
+  float c[8], s[8];
+  __device__ __forceinline__ void set(const float* cos_sin, int from, int to, int d) {
+    const f32x4* a = (const f32x4*)(cos_sin + ((long)from * 64 + d) * 2);
+    const f32x4* b = (const f32x4*)(cos_sin + ((long)to * 64 + d) * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 x = a[i], y = b[i];
+      c[2 * i] = fmaf(y[0], x[0], y[1] * x[1]);
+      s[2 * i] = fmaf(y[1], x[0], -(y[0] * x[1]));
+      c[2 * i + 1] = fmaf(y[2], x[2], y[3] * x[3]);
+      s[2 * i + 1] = fmaf(y[3], x[2], -(y[2] * x[3]));
+    }
+  }
+  __device__ __forceinline__ void apply(Row& r) const {
+    bf16x8 lo = __builtin_bit_cast(bf16x8, r.lo), hi = __builtin_bit_cast(bf16x8, r.hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = (float)lo[i], y = (float)hi[i];
+      lo[i] = f2bf(fmaf(x, c[i], -(y * s[i])));
+      hi[i] = f2bf(fmaf(y, c[i], x * s[i]));
+    }
+    r.lo = __builtin_bit_cast(u32x4, lo);
+    r.hi = __builtin_bit_cast(u32x4, hi);
+  }
+};
+
+// places of `keep` that are set among 8 from p (which need not be aligned)
+__device__ __forceinline__ int set_of_8(const uint8_t* p) {
+  uint64_t x;
+  __builtin_memcpy(&x, p, 8);
+  const uint64_t low = 0x7f7f7f7f7f7f7f7full;
+  return __popcll((((x & low) + low) | x) & ~low);
+}
+
+// Into other pages: a workgroup takes 256 / TPT consecutive places of one sequence, counts the kept ones before them, and
+// moves them in the layers and heads of its share (blockIdx.z): the turn's numbers are formed once for all of them.
+template <int TPT, bool TURN>
+__global__ __launch_bounds__(256) void compact_apart_kernel(Cache k, Cache v, Sequences s, int heads, int layers,
+                                                            const float* __restrict__ cos_sin) {
+  constexpr int TOK = 256 / TPT, HALF = TPT * 16;
+  const int seq = blockIdx.y, tid = threadIdx.x, t = tid / TPT, part = tid % TPT;
+  const int len = length_of(s, seq), p0 = blockIdx.x * TOK, place = p0 + t;
+  const bool last = p0 + TOK >= len;      // of the sequence's workgroups
+  if (p0 >= len && p0 > 0) return;
+  const uint8_t* keep = s.keep + seq * s.keep_stride;
+  __shared__ int count[4];
+  __shared__ uint8_t set[TOK];
+  int before = 0;
+  for (int j = tid * 8; j < p0; j += 256 * 8) before += set_of_8(keep + j);   // p0 is a multiple of 8
+  const bool kept = place < len && keep[place] != 0;
+  if (part == 0) set[t] = kept;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+  if ((tid & 63) == 0) count[tid >> 6] = before;
+  __syncthreads();
+  int to = count[0] + count[1] + count[2] + count[3];
+  if (last && blockIdx.z == 0 && tid == 0) {
+    int n = to;
+    for (int j = 0; j < TOK; ++j) n += set[j];
+    s.new_lens[seq] = n;
+  }
+  if (!kept) return;
+  for (int j = 0; j < t; ++j) to += set[j];
+  const int from_page = s.tables[(long)seq * s.table_stride + place / PAGE], to_page = s.to[(long)seq * s.to_stride + to / PAGE];
+  if ((unsigned)from_page >= (unsigned)s.num_pages || (unsigned)to_page >= (unsigned)s.num_pages) return;
+  Turn turn;
+  const bool turned = TURN && to != place;
+  if (turned) turn.set(cos_sin, place, to, part * 8);
+  const long inside_from = (long)(place % PAGE) * 2 * HALF + part * 16, inside_to = (long)(to % PAGE) * 2 * HALF + part * 16;
+  const int all = heads * layers;
+  for (int i = blockIdx.z; i < all; i += gridDim.z) {
+    const int h = i % heads, layer = i / heads;
+    const char* kf = k.p + layer * k.layer + h * k.head + from_page * k.page + inside_from;
+    const char* vf = v.p + layer * v.layer + h * v.head + from_page * v.page + inside_from;
+    Row a = load_row(kf, HALF);
+    const Row b = load_row(vf, HALF);
+    if (turned) turn.apply(a);
+    store_row(k.p + layer * k.layer + h * k.head + to_page * k.page + inside_to, HALF, a);
+    store_row(v.p + layer * v.layer + h * v.head + to_page * v.page + inside_to, HALF, b);
+  }
+}
+
+// In place: one workgroup moves all of a sequence's tokens of one head, 1024 / TPT places after the other.  A place n takes the
+// token of a place p >= n, so once the workgroup has read its places no later read meets what it writes.
+template <int TPT, bool TURN>
+__global__ __launch_bounds__(1024) void compact_inside_kernel(Cache k, Cache v, Sequences s, int heads,
+                                                              const float* __restrict__ cos_sin) {
+  constexpr int TOK = 1024 / TPT, HALF = TPT * 16;
+  const int seq = blockIdx.y, h = blockIdx.x % heads, layer = blockIdx.x / heads;
+  const int tid = threadIdx.x, t = tid / TPT, part = tid % TPT;
+  const int len = length_of(s, seq);
+  const uint8_t* keep = s.keep + seq * s.keep_stride;
+  const int* table = s.tables + (long)seq * s.table_stride;
+  char* kp = k.p + layer * k.layer + h * k.head + part * 16;
+  char* vp = v.p + layer * v.layer + h * v.head + part * 16;
+  __shared__ uint8_t set[2][TOK];
+  int base = 0, side = 0;
+  for (int p0 = 0; p0 < len; p0 += TOK, side ^= 1) {
+    const int place = p0 + t;
+    bool kept = place < len && keep[place] != 0;
+    if (part == 0) set[side][t] = kept;
+    __syncthreads();
+    int to = base;
+    for (int j = 0; j < TOK; ++j) {
+      const int one = set[side][j];
+      base += one;
+      if (j < t) to += one;
+    }
+    const int from_page = kept ? table[place / PAGE] : 0, to_page = kept ? table[to / PAGE] : 0;
+    kept = kept && to != place && (unsigned)from_page < (unsigned)s.num_pages && (unsigned)to_page < (unsigned)s.num_pages;
+    Row a, b;
+    if (kept) {
+      const long in = (long)(place % PAGE) * 2 * HALF;
+      a = load_row(kp + from_page * k.page + in, HALF);
+      b = load_row(vp + from_page * v.page + in, HALF);
+      if constexpr (TURN) {
+        Turn turn;
+        turn.set(cos_sin, place, to, part * 8);
+        turn.apply(a);
+      }
+    }
+    // every wavefront's loads have come back before any writes
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kept) {
+      const long in = (long)(to % PAGE) * 2 * HALF;
+      store_row(kp + to_page * k.page + in, HALF, a);
+      store_row(vp + to_page * v.page + in, HALF, b);
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) s.new_lens[seq] = base;
+}
+
+template <int TPT, bool TURN>
+int compact(Cache k, Cache v, const Sequences& s, int n, int heads, int layers, const float* cos_sin, hipStream_t st) {
+  if (!s.to) {
+    hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN>), dim3(heads * layers, n), dim3(1024), 0, st, k, v, s, heads, cos_sin);
+    return (int)hipGetLastError();
+  }
+  constexpr int TOK = 256 / TPT;
+  const int chunks = max(1, (min(s.places, s.width * PAGE) + TOK - 1) / TOK);
+  const int shares = max(1, min(heads * layers, 2048 / max(1, chunks * n)));
+  hipLaunchKernelGGL((compact_apart_kernel<TPT, TURN>), dim3(chunks, n, shares), dim3(256), 0, st, k, v, s, heads, layers, cos_sin);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+// Pages src[i] copied to dst[i] (host arrays), the first tokens[i] rows of every head in every layer.  No page may be in dst
+// twice or in both, which the caller has checked.  strides: bytes between layers, pages and heads of K, then of V.
+P2P_API int p2p_copy_pages(void* k, void* v, const long* strides, int layers, int heads, int num_pages, int row_bytes,
+                           const int* src, const int* dst, const int* tokens, int n, hipStream_t stream) {
+  if (layers < 1 || heads < 1 || row_bytes < 16 || row_bytes % 16 || n < 0) return (int)hipErrorInvalidValue;
+  const Cache ck = {(char*)k, strides[0], strides[1], strides[2]}, cv = {(char*)v, strides[3], strides[4], strides[5]};
+  for (int i = 0; i < n; ++i)
+    if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages || tokens[i] < 0 || tokens[i] > PAGE)
+      return (int)hipErrorInvalidValue;
+  for (int i = 0; i < n;) {
+    Pairs pairs;
+    int m = 0;
+    for (; i < n && m < PAIRS; ++i) {
+      if (src[i] == dst[i] || tokens[i] == 0) continue;
+      pairs.src[m] = src[i];
+      pairs.dst[m] = dst[i];
+      pairs.tokens[m++] = (uint8_t)tokens[i];
+    }
+    if (m == 0) break;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(heads * layers * m, 2), dim3(256), 0, stream, ck, cv, pairs, heads, layers, row_bytes);
+    if (int e = (int)hipGetLastError()) return e;
+  }
+  return 0;
+}
+
+// Kept tokens of n sequences to the front of their tables (to null) or of other pages; new_lens[i]: how many.  cos_sin
+// (bf16 rows of 128 only): keys turned from their old places to their new ones.
+P2P_API int p2p_compact_pages(void* k, void* v, const long* strides, int layers, int heads, int num_pages, int row_bytes,
+                              const int* tables, int table_stride, int width, const int* to, int to_stride, const int* lens,
+                              const void* keep, long keep_stride, int places, int n, const float* cos_sin, int* new_lens,
+                              hipStream_t stream) {
+  if (layers < 1 || heads < 1 || n < 1 || width < 0 || places < 0) return (int)hipErrorInvalidValue;
+  if (cos_sin && row_bytes != 256) return (int)hipErrorInvalidValue;
+  const Cache ck = {(char*)k, strides[0], strides[1], strides[2]}, cv = {(char*)v, strides[3], strides[4], strides[5]};
+  const Sequences s = {tables, to, lens, (const uint8_t*)keep, width, table_stride, to_stride, places, num_pages, keep_stride,
+                       new_lens};
+  switch (row_bytes) {
+    case 128: return compact<4, false>(ck, cv, s, n, heads, layers, nullptr, stream);
+    case 256:
+      return cos_sin ? compact<8, true>(ck, cv, s, n, heads, layers, cos_sin, stream)
+                     : compact<8, false>(ck, cv, s, n, heads, layers, nullptr, stream);
+    case 512: return compact<16, false>(ck, cv, s, n, heads, layers, nullptr, stream);
+  }
+  return (int)hipErrorInvalidValue;
+}

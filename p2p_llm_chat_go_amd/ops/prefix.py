@@ -1,0 +1,168 @@
+"""Attention of rows whose sequences begin with the same pages (csrc/kernels/prefix_attention.hip).
+
+:func:`paged_attention` reads a row's keys once per row.  Where a batch's sequences share their first pages (a system
+prompt, a thread that several replies are drawn from; ``KVCache.fork`` makes such sequences), :func:`prefix_attention` reads
+those once for all rows of the group, and a sequence's own pages once for the rows of that sequence.  Rows are as there: one
+token each, of a decode step (one row per sequence) or of prompts (consecutive rows per sequence), with a block-table row
+and a context length.
+"""
+from __future__ import annotations
+
+import dataclasses
+import math
+import operator
+
+import torch
+
+from . import _lib
+from .attention import HEAD_DIM, PAGE, paged_attention_ref
+
+ROWS = 32          # (row, head) pairs of a workgroup
+
+
+@dataclasses.dataclass(frozen=True)
+class PrefixPlan:
+    """How a batch's rows and pages are cut into works: host data of :func:`prefix_plan`, on the device once."""
+    rows: int
+    n_heads: int
+    n_kv: int
+    max_ctx: int
+    tables: int            # block tables it reads
+    parts: int             # results of parts, over all rows
+    works: torch.Tensor    # int32 [n, 8]
+    base: torch.Tensor     # int32 [rows + 1]: parts of the rows before
+    row_tables: torch.Tensor   # int32 [rows]
+
+
+def _int(x, what: str) -> int:
+    try:
+        return operator.index(x)
+    except TypeError:
+        raise ValueError("prefix_plan: %s must be whole numbers, got %r" % (what, x)) from None
+
+
+def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None) -> PrefixPlan:
+    """A plan for batches of ``sum(rows)`` query rows.
+
+    groups: (rows, pages) of every group, in the order of the rows: the next ``rows`` rows, whose block tables begin with the
+    same ``pages`` pages (0: they share nothing).  seqs: every row's block-table row (rows of one sequence one after the
+    other); None: row r has row r, as in a decode step.  max_ctx: the longest context that the plan is used for.  Context
+    lengths are not part of it: a decode step's plan serves its batch until a sequence joins or leaves."""
+    n_heads, n_kv, max_ctx = _int(n_heads, "n_heads"), _int(n_kv, "n_kv"), _int(max_ctx, "max_ctx")
+    if n_kv < 1 or n_heads < n_kv or n_heads % n_kv or n_heads // n_kv > ROWS:
+        raise ValueError("prefix_plan: %d query heads on %d kv heads (1 to %d each)" % (n_heads, n_kv, ROWS))
+    if max_ctx < 1:
+        raise ValueError("prefix_plan: max_ctx must be positive, got %d" % max_ctx)
+    groups = [(_int(r, "rows"), _int(p, "pages")) for r, p in groups]
+    pages_max = -(-max_ctx // PAGE)
+    for r, p in groups:
+        if r < 1 or p < 0 or p > pages_max:
+            raise ValueError("prefix_plan: a group of %d rows that share %d pages (contexts up to %d)" % (r, p, max_ctx))
+    R = sum(r for r, _ in groups)
+    if R < 1:
+        raise ValueError("prefix_plan: no rows")
+    seqs = list(range(R)) if seqs is None else [_int(s, "seqs") for s in (seqs.tolist() if isinstance(seqs, torch.Tensor) else seqs)]
+    if len(seqs) != R or min(seqs) < 0:
+        raise ValueError("prefix_plan: seqs must give a block table (0 ..) to each of the %d rows" % R)
+
+    tile = ROWS // (n_heads // n_kv)     # rows of a work
+    shared, owned, r0 = [], [], 0        # (first row, rows, table, first page, last page + 1)
+    for n, p in groups:
+        r1 = r0 + n
+        if seqs[r0] == seqs[r1 - 1] and len(set(seqs[r0:r1])) == 1:
+            p = 0                        # one sequence shares with nobody
+        if p:
+            shared += [[(a, min(tile, r1 - a), seqs[r0], 0, p) for a in range(r0, r1, tile)]]
+        a = r0
+        while a < r1 and p < pages_max:
+            b = a + 1
+            while b < r1 and b - a < tile and seqs[b] == seqs[a]:
+                b += 1
+            owned.append((a, b - a, seqs[a], p, pages_max))
+            a = b
+        r0 = r1
+    parts_of = lambda blocks, pages: max(1, min(-(-pages // 2), 1024 // max(1, blocks * n_kv)))
+    works, count = [], [0] * R
+    blocks = sum(len(s) for s in shared)
+    for tiles in shared:
+        C = parts_of(blocks, tiles[0][4])
+        for c in range(C):
+            works += [(a, n, t, p0, p1, c, C, 0) for a, n, t, p0, p1 in tiles]
+        for a, n, *_ in tiles:
+            count[a:a + n] = [C] * n
+    for a, n, t, p0, p1 in owned:
+        C = parts_of(len(owned), p1 - p0)
+        works += [(a, n, t, p0, p1, c, C, count[a]) for c in range(C)]
+        count[a:a + n] = [count[a] + C] * n
+    base = [0]
+    for n in count:
+        base.append(base[-1] + n)
+    dev = torch.device(device)
+    flat = [x for w in works for x in w] + seqs + base
+    flat = torch.tensor(flat, dtype=torch.int32).to(dev)
+    n = 8 * len(works)
+    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, base[-1], flat[:n].view(-1, 8), flat[n + R:], flat[n:n + R])
+
+
+def prefix_workspace(plan: PrefixPlan) -> tuple:
+    """(parts' outputs, parts' maxima and sums) for :func:`prefix_attention`; a launch uses them until it ends, so calls
+    that may run at once (on several streams, in several graphs) take one each."""
+    dev = plan.works.device
+    return (torch.empty(plan.parts * plan.n_heads * HEAD_DIM, device=dev, dtype=torch.float32),
+            torch.empty(plan.parts * plan.n_heads * 2, device=dev, dtype=torch.float32))
+
+
+def _check(ok: bool, why: str):
+    if not ok:
+        raise ValueError("prefix_attention: " + why)
+
+
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                     ctx_lens: torch.Tensor, plan: PrefixPlan, out: torch.Tensor | None = None,
+                     workspace: tuple | None = None, scale: float | None = None) -> torch.Tensor:
+    """q: [R, n_heads * 128] bf16 -> out [R, n_heads * 128] bf16, as :func:`paged_attention` with the plan's tables.
+
+    Row r attends the first ``min(ctx_lens[r], plan.max_ctx)`` tokens of its block table; a row that sees none is 0.  Rows
+    behind the plan's are not read or written.  A group's shared pages are read through its first row's table.  Block
+    tables hold pages of the cache; others read page 0 or the last one."""
+    R, n_heads, n_kv = plan.rows, plan.n_heads, plan.n_kv
+    width = n_heads * HEAD_DIM
+    _check(q.dim() == 2 and q.dtype == torch.bfloat16 and q.shape[0] >= R and q.shape[1] == width
+           and (q.stride(1) == 1 or width == 1), "q must be bf16 [%d or more, %d], rows contiguous" % (R, width))
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _check(c.dim() == 4 and c.shape[1:] == (n_kv, PAGE, HEAD_DIM) and c.dtype == torch.bfloat16 and c.is_contiguous()
+               and c.shape[0] > 0, "%s must be bf16 [pages, %d, %d, %d], contiguous" % (name, n_kv, PAGE, HEAD_DIM))
+    _check(k_cache.shape == v_cache.shape, "k_cache and v_cache differ in shape")
+    _check(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
+           and block_tables.shape[0] >= plan.tables and block_tables.shape[1] * PAGE >= plan.max_ctx,
+           "block_tables must be int32 [%d or more, pages of %d tokens]" % (plan.tables, plan.max_ctx))
+    _check(ctx_lens.dim() == 1 and ctx_lens.dtype == torch.int32 and ctx_lens.shape[0] >= R and ctx_lens.stride(0) == 1,
+           "ctx_lens must be int32 [%d or more]" % R)
+    if scale is None:
+        scale = 1.0 / math.sqrt(HEAD_DIM)
+    _check(0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
+    if out is None:
+        out = torch.empty(q.shape[0], width, device=q.device, dtype=q.dtype)
+    _check(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width
+           and out.stride(1) == 1, "out must be bf16 [%d or more, %d], rows contiguous" % (R, width))
+    given = (q, k_cache, v_cache, block_tables, ctx_lens, plan.works, out) + tuple(workspace or ())
+    _check(all(t.device == q.device for t in given), "tensors and plan must be on one device")
+    if q.device.type != "cuda":
+        ctx = ctx_lens[:R].clamp(0, plan.max_ctx)
+        some = ctx > 0
+        paged_attention_ref(q[:R], k_cache, v_cache, block_tables, plan.row_tables, ctx.clamp(min=1), n_heads, n_kv, scale,
+                            out[:R])
+        out[:R] = torch.where(some[:, None], out[:R], 0)
+        return out
+    if workspace is None:
+        workspace = prefix_workspace(plan)
+    po, pml = workspace
+    _check(po.dtype == pml.dtype == torch.float32 and po.is_contiguous() and pml.is_contiguous()
+           and po.numel() >= plan.parts * width and pml.numel() >= plan.parts * n_heads * 2, "workspace is not this plan's")
+    with _lib.device_of(q):
+        _lib.check(_lib.lib().p2p_prefix_attention(
+            q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_tables.data_ptr(),
+            block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx, plan.works.data_ptr(), plan.works.shape[0],
+            plan.base.data_ptr(), plan.row_tables.data_ptr(), R, n_heads, n_kv, HEAD_DIM, float(scale), out.data_ptr(),
+            out.stride(0), po.data_ptr(), pml.data_ptr(), _lib.stream_ptr(q.device)), "prefix_attention")
+    return out
