@@ -29,43 +29,267 @@ __device__ __forceinline__ int kperm(int rho) {  // S^T row rho -> key within th
   return 16 * s + 8 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
 }
 
-// Four wavefronts, each with its own 32 keys at a time against the same 32 (row, head) pairs: S^T = K . Q^T and
-// O^T += V^T . P^T in 32x32x16 products, a pair per lane, as in flash_prefill2_kernel.  K and V come by LDS DMA into the
-// wavefront's own LDS, the next K while this one's weights are formed, the next V behind the second product; no barrier
-// until the four meet at the end.  P is rounded to bf16 for the product (relative 2^-9, as in flash_prefill.hip: what a
-// value's weight is off by); scores, maxima, sums and O are fp32.
-constexpr int NW = 4, KT = 32, ROWS = 32;
+constexpr int NW = 4, ROWS = 32;
+constexpr int PG = PAGE * HD;                    // numbers of a page's K (V)
 
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(
-    const bf16* __restrict__ q, int ldq, const bf16* __restrict__ kc, const bf16* __restrict__ vc, int num_pages,
-    const int* __restrict__ bt, int bt_stride, const int* __restrict__ ctx_lens, int max_ctx, const Work* __restrict__ works,
-    int n_works, const int* __restrict__ base, int Hkv, int G, float scale_log2, float* __restrict__ part_o, float2* __restrict__ part_ml) {
-  __shared__ __attribute__((aligned(16))) bf16 lds[NW][2][KT * HD];   // K and V of every wavefront; its O at the end
-  __shared__ float2 sml[NW][ROWS];
-  const int b = xcd_remap(blockIdx.x, n_works * Hkv);
-  const Work W = works[b / Hkv];
-  const int kvh = b % Hkv;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int r32 = lane & 31, hh = lane >> 5;
-  const int pairs = W.n * G, pair = min(r32, pairs - 1), row = W.row0 + pair / G, head = kvh * G + pair % G;
-  const int lim = min(ctx_lens[row], max_ctx);   // keys that this lane's row sees
-  int most = lim;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
-  most = __builtin_amdgcn_readfirstlane(most);
-  const int np = max(0, (min(most, W.page1 * PAGE) + PAGE - 1) / PAGE - W.page0);   // pages that some row sees
+struct Args {
+  const bf16 *q, *kc, *vc;
+  const int *bt, *ctx_lens, *base;
+  float* part_o;
+  float2* part_ml;
+  int ldq, num_pages, bt_stride, max_ctx, Hkv, G;
+  float scale_log2;
+};
+
+// A workgroup's share of a work: pages first .. end - 1, of whose keys the last that some row sees is `last`.
+struct Share {
+  int first, end, last;
+};
+__device__ __forceinline__ Share share_of(const Work& W, int most) {
+  const int np = max(0, (min(most, W.page1 * PAGE) + PAGE - 1) / PAGE - W.page0);
   const int first = W.page0 + (int)((long)np * W.part / W.of), end = W.page0 + (int)((long)np * (W.part + 1) / W.of);
-  const int last = min(most, end * PAGE) - 1;             // last key
-  const int u0 = first * 2 + w, u1 = first < end ? last / KT + 1 : 0;   // units of 32 keys, this wavefront's every fourth
+  return {first, end, min(most, end * PAGE) - 1};
+}
+__device__ __forceinline__ int most_of(const Args& A, const Work& W, int lane) {   // keys that some row sees
+  int most = 0;
+  for (int r = lane; r < W.n; r += 64) most = max(most, min(A.ctx_lens[W.row0 + r], A.max_ctx));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  return __builtin_amdgcn_readfirstlane(most);
+}
+__device__ __forceinline__ int page_at(const Args& A, const int* btr, int at) {
+  return min(max(btr[at], 0), A.num_pages - 1);
+}
 
-  const size_t page_sz = (size_t)Hkv * PAGE * HD, head_off = (size_t)kvh * PAGE * HD;
-  const int* btr = bt + (size_t)W.table * bt_stride;
-  const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(&lds[w][0][0]));
+// Q^T operand of a lane's (row, head) pair: k-step s covers numbers 16 s .. 16 s + 15, lane half hh has 8 hh .. 8 hh + 7
+__device__ __forceinline__ void load_q(const Args& A, int row, int head, int hh, bf16x8 (&qf)[8]) {
+  const bf16* qp = A.q + (size_t)row * A.ldq + (size_t)head * HD + 8 * hh;
+#pragma unroll
+  for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const bf16x8_u*>(qp + 16 * s);
+#pragma unroll
+  for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(qf[s]));   // loaded before the copies are counted
+}
+
+// A lane's O (numbers 32 db + 8 g4 + 4 hh + 0 .. 3 of pair r32) as rows of 512 bytes in LDS, 16-byte piece p at p ^ r32
+__device__ __forceinline__ void put_rows(float* so, const f32x16 (&o)[4], int r32, int hh) {
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      *reinterpret_cast<f32x4*>(so + r32 * HD + (((8 * db + 2 * g4 + hh) ^ r32) << 2)) =
+          f32x4{o[db][4 * g4], o[db][4 * g4 + 1], o[db][4 * g4 + 2], o[db][4 * g4 + 3]};
+}
+__device__ __forceinline__ f32x4 get_row(const float* so, int pair, int piece) {
+  return *reinterpret_cast<const f32x4*>(so + pair * HD + ((piece ^ pair) << 2));
+}
+
+__device__ __forceinline__ size_t part_at(const Args& A, const Work& W, int kvh, int pair) {
+  return ((size_t)(A.base[W.row0 + pair / A.G] + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds4_t;
+// eight keys of a V^T operand from rows of 256 bytes, 16-byte piece p of row r at p ^ 4 (r & 3): `p` is this lane's place
+__device__ __forceinline__ bf16x8 read_v8(const bf16* p) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(p + 4 * HD));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ---- up to 128 pairs ----
+// A wavefront has 32 pairs, a workgroup's four share the pages: K and V of a page come by LDS DMA, two stages each, and a
+// page's exponentials run between the products of the page before with V, as in flash_prefill2_kernel (whose layouts these
+// are).  P is rounded to bf16 for the product (relative 2^-9: what a value's weight is off by); scores, maxima, sums and O
+// are fp32.
+__device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh, bf16* lds, int w, int lane) {
+  const int r32 = lane & 31, hh = lane >> 5;
+  const Share S = share_of(W, most_of(A, W, lane));
+  const int pairs = W.n * A.G, mine = w * 32 + r32, pair = min(mine, pairs - 1), row = W.row0 + pair / A.G;
+  const int lim = min(A.ctx_lens[row], A.max_ctx);
+  f32x16 o[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (S.first < S.end) {
+    const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
+    const int* btr = A.bt + (size_t)W.table * A.bt_stride;
+    constexpr int CP = 16 / NW;
+    const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds)) + w * 1024;
+    const int cr = 4 * w + (lane >> 4), cp = lane & 15;
+    // an instruction takes four rows of 256 bytes; rows past the last key (whatever they hold) are that key's again
+    auto copy = [&](const bf16* pool, int kt, int page, unsigned dst, bool is_v) {
+      const bf16* from = pool + (size_t)page * page_sz + head_off;
+      const int top = S.last - kt * PAGE;
+#pragma unroll
+      for (int i = 0; i < CP; ++i) {
+        const int r = cr + 4 * NW * i;
+        ldsp::dma_lds16(from, min(r, top) * (HD * 2) + ((cp ^ (is_v ? 4 * (r & 3) : r & 15)) << 4), dst + i * NW * 1024);
+      }
+    };
+    auto copy_k = [&](int kt, int page) { copy(A.kc, kt, page, l0 + (kt & 1) * (PG * 2), false); };
+    auto copy_v = [&](int kt, int page) { copy(A.vc, kt, page, l0 + (2 + (kt & 1)) * (PG * 2), true); };
+    auto page_of = [&](int kt) { return page_at(A, btr, min(kt, S.end - 1)); };
+    int p0 = page_of(S.first), p1 = page_of(S.first + 1);   // pages kt and kt + 1
+    bf16x8 qf[8];
+    load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
+    copy_k(S.first, p0);
+
+    const int krow = kperm(r32), L = lane & 15;
+    const bf16* kl = lds + krow * HD;
+    const bf16* vl = lds + 2 * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1);
+    const int vp = 2 * ((lane >> 4) & 1) + ((L >> 1) & 1);
+    auto read_k = [&](int st, int kh, int s) {
+      return *reinterpret_cast<const bf16x8*>(kl + st * PG + 32 * kh * HD + (((2 * s + hh) ^ (krow & 15)) << 3));
+    };
+    // V^T of numbers 32 db + r32, keys 32 kh + 16 s2 + 8 hh + 0 .. 7
+    auto read_v = [&](int st, int db, int kh, int s2) {
+      return read_v8(vl + st * PG + (32 * kh + 16 * s2) * HD + ((((db ^ (L >> 2)) << 2) | vp) << 3));
+    };
+    f32x16 sc[2];
+    bf16x8 pf[2][2];   // P^T of the page before
+    // O^T += V^T . P^T of page `of` in eight pairs of products; LDS reads go out a pair ahead, and between them runs `work`
+    auto second_product = [&](int of, auto&& work) {
+      const int st = of & 1;
+      bf16x8 vf[2][2];
+      auto read_v2 = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vf[j & 1][i] = read_v(st, j >> 1, j & 1, i);
+      };
+      read_v2(0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < 7) read_v2(j + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          o[j >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 1][i], pf[j & 1][i], o[j >> 1], 0, 0, 0);
+        work(j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int kt = S.first; kt < S.end; ++kt) {
+      // K of this page and V of the one before have landed; every wave is past the last page's K and the V before it
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      copy_v(kt, p0);
+      if (kt + 1 < S.end) copy_k(kt + 1, p1);
+      p0 = p1;
+      p1 = page_of(kt + 2);
+      {
+        bf16x8 kf[2][2];
+        auto read_k2 = [&](int s) {
+#pragma unroll
+          for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = read_k(kt & 1, kh, s);
+        };
+        read_k2(0);
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[kh][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          if (s < 7) read_k2(s + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int kh = 0; kh < 2; ++kh)
+            sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s & 1][kh], qf[s], sc[kh], 0, 0, 0);
+        }
+      }
+      // Keys of register rr of half kh: 16 (rr >> 3) + 8 hh + (rr & 7).  O and l are rescaled only when some row's maximum grew
+      // by more than 2^8 (wave-uniform): until then weights stay below 2^8, as exact in bf16 as below 1.
+      constexpr float RESCALE_THR = 8.f;
+      const int k0 = kt * PAGE;
+      if (__any(k0 + PAGE > lim)) {
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int rr = 0; rr < 16; ++rr)
+            if (k0 + 32 * kh + 16 * (rr >> 3) + 8 * hh + (rr & 7) >= lim) sc[kh][rr] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) mx = fmaxf(mx, sc[kh][rr]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const bool rescale = __any((mx - m) * A.scale_log2 > RESCALE_THR);
+      float alpha = 1.f;
+      if (rescale) {
+        const float mn = fmaxf(m, mx);
+        alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * A.scale_log2);   // (no key yet: -inf both)
+        m = mn;
+        l *= alpha;
+      }
+      const float mc = m == -INFINITY ? 0.f : m * A.scale_log2;
+      float ps = 0.f;
+      bf16x8 pn[2][2];
+      auto exps = [&](int j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int kh = j >> 2, rr = (j & 3) * 4 + e;
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr], A.scale_log2, -mc));
+          ps += p;
+          pn[kh][rr >> 3][rr & 7] = f2bf(p);
+        }
+      };
+      if (kt > S.first) {
+        second_product(kt - 1, exps);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) exps(j);
+      }
+      l += ps;
+      if (rescale) {   // (O has the page before by now, which the old maximum scaled)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) o[db] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[i >> 1][i & 1] = pn[i >> 1][i & 1];
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    second_product(S.end - 1, [](int) {});
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  // the wavefront's rows to LDS and from there in whole rows
+  float* so = reinterpret_cast<float*>(lds) + w * (32 * HD);
+  put_rows(so, o, r32, hh);
+  if (hh == 0 && mine < pairs)
+    A.part_ml[part_at(A, W, kvh, mine)] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int p = 2 * i + hh;
+    if (w * 32 + p < pairs)
+      *reinterpret_cast<f32x4*>(A.part_o + part_at(A, W, kvh, w * 32 + p) * HD + 4 * r32) = get_row(so, p, r32);
+  }
+}
+
+// ---- up to 32 pairs ----
+// Four wavefronts, each with its own 32 keys at a time against the same pairs.  K and V come by LDS DMA into the wavefront's
+// own LDS, the next K while this one's weights are formed, the next V behind the second product; no barrier until the four
+// meet at the end.
+constexpr int KT = 32;
+
+__device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, float2 (*sml)[ROWS], int tid, int w,
+                                         int lane) {
+  bf16* lds = lds_all + w * (2 * KT * HD);   // K and V; O at the end
+  const int r32 = lane & 31, hh = lane >> 5;
+  const int pairs = W.n * A.G, pair = min(r32, pairs - 1), row = W.row0 + pair / A.G;
+  const int lim = min(A.ctx_lens[row], A.max_ctx);
+  const Share S = share_of(W, most_of(A, W, lane));
+  const int u0 = S.first * 2 + w, u1 = S.first < S.end ? S.last / KT + 1 : 0;   // units of 32 keys, this wavefront's every fourth
+
+  const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
+  const int* btr = A.bt + (size_t)W.table * A.bt_stride;
+  const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds));
   const int cr = lane >> 4, cp = lane & 15;
-  // an instruction takes four rows of 256 bytes; rows past the last key (whatever they hold) are that key's again
   auto copy = [&](const bf16* pool, int u, int page, bool is_v) {
     const bf16* from = pool + (size_t)page * page_sz + head_off + (size_t)(u % 2) * KT * HD;
-    const int top = last - u * KT;
+    const int top = S.last - u * KT;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = cr + 4 * i;
@@ -73,16 +297,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
                       l0 + is_v * (KT * HD * 2) + i * 1024);
     }
   };
-  auto page_of = [&](int u) { return min(max(btr[min(u, u1 - 1) / 2], 0), num_pages - 1); };
+  auto page_of = [&](int u) { return page_at(A, btr, min(u, u1 - 1) / 2); };
 
   bf16x8 qf[8];
-  {
-    const bf16* qp = q + (size_t)row * ldq + (size_t)head * HD + 8 * hh;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const bf16x8_u*>(qp + 16 * s);
-  }
-#pragma unroll
-  for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(qf[s]));   // loaded before the copies are counted
+  load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
   f32x16 o[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -91,22 +309,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   float m = -INFINITY, l = 0.f;
 
   const int krow = kperm(r32), L = lane & 15;
-  const bf16* kl = &lds[w][0][krow * HD];
-  const bf16* vl = &lds[w][1][(8 * hh + (L >> 2)) * HD + 4 * (L & 1)];
+  const bf16* kl = lds + krow * HD;
+  const bf16* vl = lds + KT * HD + (8 * hh + (L >> 2)) * HD + 4 * (L & 1);
   const int vp = 2 * ((lane >> 4) & 1) + ((L >> 1) & 1);
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) s16x4* lds4_t;
   auto read_v = [&](int db, int s2) {   // V^T of numbers 32 db + r32, keys 16 s2 + 8 hh + 0 .. 7
-    const bf16* p = vl + 16 * s2 * HD + ((((db ^ (L >> 2)) << 2) | vp) << 3);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(p + 4 * HD));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return read_v8(vl + 16 * s2 * HD + ((((db ^ (L >> 2)) << 2) | vp) << 3));
   };
 
   if (u0 < u1) {
     int page = page_of(u0);
-    copy(kc, u0, page, false);
-    copy(vc, u0, page, true);
+    copy(A.kc, u0, page, false);
+    copy(A.vc, u0, page, true);
     page = page_of(u0 + NW);
     for (int u = u0; u < u1; u += NW) {
       const bool more = u + NW < u1;
@@ -120,7 +333,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(kf[s]));
-        if (more) copy(kc, u + NW, page, false);
+        if (more) copy(A.kc, u + NW, page, false);
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
@@ -137,14 +350,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       for (int rr = 1; rr < 16; ++rr) mx = fmaxf(mx, sc[rr]);
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float mn = fmaxf(m, mx);
-      const float ms = mn == -INFINITY ? 0.f : mn * scale_log2;    // no key yet: weights 0
-      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale_log2);
+      const float ms = mn == -INFINITY ? 0.f : mn * A.scale_log2;    // no key yet: weights 0
+      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * A.scale_log2);
       m = mn;
       float ps = 0.f;
       bf16x8 pf[2];
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[rr], scale_log2, -ms));
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[rr], A.scale_log2, -ms));
         ps += p;
         pf[rr >> 3][rr & 7] = f2bf(p);
       }
@@ -164,7 +377,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) asm volatile("" : "+v"(vf[db][s2]));
-      if (more) copy(vc, u + NW, page, true);
+      if (more) copy(A.vc, u + NW, page, true);
       page = page_of(u + 2 * NW);
 #pragma unroll
       for (int db = 0; db < 4; ++db)
@@ -173,19 +386,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   }
   l += __shfl_xor(l, 32, 64);
-  // the four meet: O of pair r32 as rows of 512 bytes, 16-byte piece p at p ^ r32
-  float* so = reinterpret_cast<float*>(&lds[w][0][0]);
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4) {   // registers 4 g4 ..: numbers 32 db + 8 g4 + 4 hh + 0 .. 3
-      const int piece = 8 * db + 2 * g4 + hh;
-      *reinterpret_cast<f32x4*>(so + r32 * HD + ((piece ^ r32) << 2)) =
-          f32x4{o[db][4 * g4], o[db][4 * g4 + 1], o[db][4 * g4 + 2], o[db][4 * g4 + 3]};
-    }
-  if (hh == 0) sml[w][r32] = make_float2(m == -INFINITY ? m : m * scale_log2, l);
+  put_rows(reinterpret_cast<float*>(lds), o, r32, hh);
+  if (hh == 0) sml[w][r32] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
   __syncthreads();
-  const float* all = reinterpret_cast<const float*>(lds);
+  const float* all = reinterpret_cast<const float*>(lds_all);
 #pragma unroll
   for (int i = 0; i < ROWS * 32 / (NW * 64); ++i) {
     const int at = tid + i * NW * 64, p = at >> 5, piece = at & 31;
@@ -199,14 +403,25 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     for (int x = 0; x < NW; ++x) {
       const float2 ml = sml[x][p];
       const float e = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
-      sum += *reinterpret_cast<const f32x4*>(all + x * (KT * HD) + p * HD + ((piece ^ p) << 2)) * e;
+      sum += get_row(all + x * (KT * HD), p, piece) * e;
       den = fmaf(e, ml.y, den);
     }
-    const int r = W.row0 + p / G;
-    const size_t to = ((size_t)(base[r] + W.slot + W.part) * Hkv + kvh) * G + p % G;
-    *reinterpret_cast<f32x4*>(part_o + to * HD + 4 * piece) = sum;
-    if (piece == 0) part_ml[to] = make_float2(M, den);
+    const size_t to = part_at(A, W, kvh, p);
+    *reinterpret_cast<f32x4*>(A.part_o + to * HD + 4 * piece) = sum;
+    if (piece == 0) A.part_ml[to] = make_float2(M, den);
   }
+}
+
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(
+    Args A, const Work* __restrict__ works) {
+  __shared__ __attribute__((aligned(16))) bf16 lds[4 * PG];
+  __shared__ float2 sml[NW][ROWS];
+  // heads first: with 8 kv heads an XCD has one of them, and its L2 that head's pages for all tiles
+  const int b = blockIdx.x;
+  const Work W = works[b / A.Hkv];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  if (W.n * A.G > ROWS) tile_role(A, W, b % A.Hkv, lds, w, lane);
+  else few_role(A, W, b % A.Hkv, lds, sml, tid, w, lane);
 }
 
 // One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
@@ -243,46 +458,64 @@ __device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const
   acc[1] /= l;
 }
 
-// The parts of a row: a wavefront per (row, head), two numbers per lane.
-__global__ __launch_bounds__(256) void prefix_combine_kernel(
-    const bf16* __restrict__ q, int ldq, const bf16* __restrict__ kc, const bf16* __restrict__ vc, int num_pages,
-    const int* __restrict__ bt, int bt_stride, const int* __restrict__ ctx_lens, int max_ctx, const int* __restrict__ base,
-    const int* __restrict__ tables, int R, int Hkv, int G, float scale_log2, const float* __restrict__ part_o,
-    const float2* __restrict__ part_ml, bf16* __restrict__ out, int ldo) {
-  const int Hq = Hkv * G, lane = threadIdx.x & 63;
-  const int i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  if (i >= R * Hq) return;
+// The parts of a row: WPP wavefronts per (row, head), two numbers per lane.  Many parts go to four wavefronts, which meet in
+// LDS: a wavefront has eight loads in flight.
+template <int WPP>
+__global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* __restrict__ tables, int R, bf16* __restrict__ out,
+                                                             int ldo) {
+  __shared__ float2 meet[4][64];
+  __shared__ float meet_den[4];
+  const int Hq = A.Hkv * A.G, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = blockIdx.x * (4 / WPP) + w / WPP, sub = w % WPP;
+  if (i >= R * Hq) return;    // (WPP 4: the whole workgroup)
   const int r = i / Hq, h = i % Hq;
-  const int b0 = base[r], n = base[r + 1] - b0;
+  const int b0 = A.base[r], n = A.base[r + 1] - b0;
+  const float2* ml = A.part_ml + (size_t)b0 * Hq + h;
+  const float* po = A.part_o + ((size_t)b0 * Hq + h) * HD + 2 * lane;
   float M = -INFINITY;
-  for (int c = lane; c < n; c += 64) M = fmaxf(M, part_ml[(size_t)(b0 + c) * Hq + h].x);
+  for (int c = lane; c < n; c += 64) M = fmaxf(M, ml[(size_t)c * Hq].x);
   M = wave_max(M);
   float acc[2] = {0.f, 0.f}, den = 0.f;
-  for (int c0 = 0; c0 < n; c0 += 64) {
+  for (int j0 = 0; sub + WPP * j0 < n; j0 += 64) {   // this wavefront's parts: sub + WPP j
+    const int c = sub + WPP * (j0 + lane);
     float e = 0.f;
-    if (c0 + lane < n) {
-      const float2 ml = part_ml[(size_t)(b0 + c0 + lane) * Hq + h];
-      e = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
-      den = fmaf(e, ml.y, den);
+    if (c < n) {
+      const float2 x = ml[(size_t)c * Hq];
+      e = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - M);
+      den = fmaf(e, x.y, den);
     }
-    const int nc = min(64, n - c0);
+    const int nj = min(64, (n - sub - WPP * j0 + WPP - 1) / WPP);
 #pragma unroll 8
-    for (int c = 0; c < nc; ++c) {
-      const float2 v = *reinterpret_cast<const float2*>(part_o + ((size_t)(b0 + c0 + c) * Hq + h) * HD + 2 * lane);
-      const float ec = __shfl(e, c, 64);
+    for (int j = 0; j < nj; ++j) {
+      const float2 v = *reinterpret_cast<const float2*>(po + (size_t)(sub + WPP * (j0 + j)) * Hq * HD);
+      const float ec = __shfl(e, j, 64);
       acc[0] = fmaf(ec, v.x, acc[0]);
       acc[1] = fmaf(ec, v.y, acc[1]);
     }
   }
   den = wave_sum(den);
+  if constexpr (WPP > 1) {
+    meet[w][lane] = make_float2(acc[0], acc[1]);
+    if (lane == 0) meet_den[w] = den;
+    __syncthreads();
+    if (w > 0) return;
+    acc[0] = acc[1] = den = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float2 v = meet[x][lane];
+      acc[0] += v.x;
+      acc[1] += v.y;
+      den += meet_den[x];
+    }
+  }
   if (M == -INFINITY && !(den != den)) {
     acc[0] = acc[1] = 0.f;    // no key
   } else {
     acc[0] /= den;
     acc[1] /= den;
     if (__any(!(fabsf(acc[0]) < INFINITY) || !(fabsf(acc[1]) < INFINITY)))
-      exact_pair(q + (size_t)r * ldq + (size_t)h * HD, kc, vc, bt + (size_t)tables[r] * bt_stride, num_pages,
-                 (size_t)Hkv * PAGE * HD, (size_t)(h / G) * PAGE * HD, min(ctx_lens[r], max_ctx), scale_log2, lane, acc);
+      exact_pair(A.q + (size_t)r * A.ldq + (size_t)h * HD, A.kc, A.vc, A.bt + (size_t)tables[r] * A.bt_stride, A.num_pages,
+                 (size_t)A.Hkv * PG, (size_t)(h / A.G) * PG, min(A.ctx_lens[r], A.max_ctx), A.scale_log2, lane, acc);
   }
   bf16* op = out + (size_t)r * ldo + (size_t)h * HD + 2 * lane;
   op[0] = f2bf(acc[0]);
@@ -295,17 +528,19 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(
 // tables; part_o, part_ml: base[R] * Hq * (128 | 2) floats.  Every part of every row belongs to one work.
 P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int num_pages,
                                  const int* block_tables, int bt_stride, const int* ctx_lens, int max_ctx, const int* works,
-                                 int n_works, const int* base, const int* tables, int R, int Hq, int Hkv, int head_dim, float scale,
-                                 void* out, int ldo, float* part_o, float* part_ml, hipStream_t stream) {
+                                 int n_works, const int* base, const int* tables, int R, int parts, int Hq, int Hkv,
+                                 int head_dim, float scale, void* out, int ldo, float* part_o, float* part_ml, hipStream_t stream) {
   if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0) return (int)hipErrorInvalidValue;
   const float sl2 = scale * 1.4426950408889634f;
   const int G = Hq / Hkv;
-  hipLaunchKernelGGL(prefix_attn_kernel, dim3(n_works * Hkv), dim3(NW * 64), 0, stream, (const bf16*)q, ldq,
-                     (const bf16*)k_cache, (const bf16*)v_cache, num_pages, block_tables, bt_stride, ctx_lens, max_ctx,
-                     (const Work*)works, n_works, base, Hkv, G, sl2, part_o, (float2*)part_ml);
+  const bool many = parts > 8 * R;
+  const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, base, part_o,
+                  (float2*)part_ml, ldq, num_pages, bt_stride, max_ctx, Hkv, G, sl2};
+  hipLaunchKernelGGL(prefix_attn_kernel, dim3(n_works * Hkv), dim3(NW * 64), 0, stream, A, (const Work*)works);
   if (int e = (int)hipGetLastError()) return e;
-  hipLaunchKernelGGL(prefix_combine_kernel, dim3((R * Hq + 3) / 4), dim3(256), 0, stream, (const bf16*)q, ldq,
-                     (const bf16*)k_cache, (const bf16*)v_cache, num_pages, block_tables, bt_stride, ctx_lens, max_ctx, base,
-                     tables, R, Hkv, G, sl2, part_o, (const float2*)part_ml, (bf16*)out, ldo);
+  if (many)
+    hipLaunchKernelGGL(prefix_combine_kernel<4>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R, (bf16*)out, ldo);
+  else
+    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 3) / 4), dim3(256), 0, stream, A, tables, R, (bf16*)out, ldo);
   P2P_CHECK_LAUNCH();
 }

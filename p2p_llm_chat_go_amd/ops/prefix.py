@@ -17,7 +17,9 @@ import torch
 from . import _lib
 from .attention import HEAD_DIM, PAGE, paged_attention_ref
 
-ROWS = 32          # (row, head) pairs of a workgroup
+import os
+TOTAL_SHARED=int(os.environ.get('TS','512')); TOTAL_OWN=int(os.environ.get('TO','1024'))
+FEW, MANY = 32, 128    # (row, head) pairs of a workgroup, in the kernel's two roles
 
 
 @dataclasses.dataclass(frozen=True)
@@ -49,8 +51,8 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     other); None: row r has row r, as in a decode step.  max_ctx: the longest context that the plan is used for.  Context
     lengths are not part of it: a decode step's plan serves its batch until a sequence joins or leaves."""
     n_heads, n_kv, max_ctx = _int(n_heads, "n_heads"), _int(n_kv, "n_kv"), _int(max_ctx, "max_ctx")
-    if n_kv < 1 or n_heads < n_kv or n_heads % n_kv or n_heads // n_kv > ROWS:
-        raise ValueError("prefix_plan: %d query heads on %d kv heads (1 to %d each)" % (n_heads, n_kv, ROWS))
+    if n_kv < 1 or n_heads < n_kv or n_heads % n_kv or n_heads // n_kv > FEW:
+        raise ValueError("prefix_plan: %d query heads on %d kv heads (1 to %d each)" % (n_heads, n_kv, FEW))
     if max_ctx < 1:
         raise ValueError("prefix_plan: max_ctx must be positive, got %d" % max_ctx)
     groups = [(_int(r, "rows"), _int(p, "pages")) for r, p in groups]
@@ -65,33 +67,38 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     if len(seqs) != R or min(seqs) < 0:
         raise ValueError("prefix_plan: seqs must give a block table (0 ..) to each of the %d rows" % R)
 
-    tile = ROWS // (n_heads // n_kv)     # rows of a work
+    G = n_heads // n_kv
+    few, many = FEW // G, MANY // G      # rows of a work
+    def cut(a, b):
+        """Rows a .. b - 1 as tiles."""
+        tile = few if (b - a) * G <= FEW else many
+        return [(i, min(tile, b - i)) for i in range(a, b, tile)]
     shared, owned, r0 = [], [], 0        # (first row, rows, table, first page, last page + 1)
     for n, p in groups:
         r1 = r0 + n
         if seqs[r0] == seqs[r1 - 1] and len(set(seqs[r0:r1])) == 1:
             p = 0                        # one sequence shares with nobody
         if p:
-            shared += [[(a, min(tile, r1 - a), seqs[r0], 0, p) for a in range(r0, r1, tile)]]
+            shared.append([(a, k, seqs[r0], 0, p) for a, k in cut(r0, r1)])
         a = r0
         while a < r1 and p < pages_max:
             b = a + 1
-            while b < r1 and b - a < tile and seqs[b] == seqs[a]:
+            while b < r1 and seqs[b] == seqs[a]:
                 b += 1
-            owned.append((a, b - a, seqs[a], p, pages_max))
+            owned += [(i, k, seqs[a], p, pages_max) for i, k in cut(a, b)]
             a = b
         r0 = r1
-    parts_of = lambda blocks, pages: max(1, min(-(-pages // 2), 1024 // max(1, blocks * n_kv)))
+    parts_of = lambda blocks, pages, total: max(1, min(-(-pages // 2), total // max(1, blocks * n_kv)))
     works, count = [], [0] * R
     blocks = sum(len(s) for s in shared)
     for tiles in shared:
-        C = parts_of(blocks, tiles[0][4])
+        C = parts_of(blocks, tiles[0][4], TOTAL_SHARED)
         for c in range(C):
             works += [(a, n, t, p0, p1, c, C, 0) for a, n, t, p0, p1 in tiles]
         for a, n, *_ in tiles:
             count[a:a + n] = [C] * n
     for a, n, t, p0, p1 in owned:
-        C = parts_of(len(owned), p1 - p0)
+        C = parts_of(len(owned), p1 - p0, TOTAL_OWN)
         works += [(a, n, t, p0, p1, c, C, count[a]) for c in range(C)]
         count[a:a + n] = [count[a] + C] * n
     base = [0]
@@ -163,6 +170,6 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         _lib.check(_lib.lib().p2p_prefix_attention(
             q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_tables.data_ptr(),
             block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx, plan.works.data_ptr(), plan.works.shape[0],
-            plan.base.data_ptr(), plan.row_tables.data_ptr(), R, n_heads, n_kv, HEAD_DIM, float(scale), out.data_ptr(),
+            plan.base.data_ptr(), plan.row_tables.data_ptr(), R, plan.parts, n_heads, n_kv, HEAD_DIM, float(scale), out.data_ptr(),
             out.stride(0), po.data_ptr(), pml.data_ptr(), _lib.stream_ptr(q.device)), "prefix_attention")
     return out

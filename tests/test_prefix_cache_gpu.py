@@ -72,6 +72,15 @@ def test_prefix_attention_of_decode_rows(Hq, Hkv, groups, own):
     _check(_run(q, k, v, table, ctx, plan), want, bound)
 
 
+@pytest.mark.parametrize("groups,own", [([(2, 560)], 9), ([(40, 150)], 3), ([(1, 0), (2, 700)], 2)])
+def test_prefix_attention_in_many_parts(groups, own):
+    """One kv head: up to some 300 parts of a row."""
+    q, k, v, table, seqs, ctx, rows, most = _batch(groups, 8, 1, own, own)
+    plan = ops.prefix_plan(rows, 8, 1, most, DEV)
+    want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 1, 1 / math.sqrt(D), most)
+    _check(_run(q, k, v, table, ctx, plan), want, bound)
+
+
 @pytest.mark.parametrize("Hq,Hkv", [(8, 2), (4, 4), (8, 1), (3, 1)])
 @pytest.mark.parametrize("groups,own,tokens", [([(3, 2)], 44, 44), ([(2, 4), (3, 1)], 100, 17), ([(1, 5)], 200, 130),
                                                ([(9, 1)], 64, 2)])
