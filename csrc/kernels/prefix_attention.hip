@@ -57,7 +57,17 @@ __device__ __forceinline__ int most_of(const Args& A, const Work& W, int lane) {
   for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
   return __builtin_amdgcn_readfirstlane(most);
 }
-__device__ __forceinline__ int page_at(const Args& A, const int* btr, int at) {
+__device__ __forceinline__ int least_of(int lim) {   // of the wavefront's 32 rows
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lim = min(lim, __shfl_xor(lim, o, 64));
+  return __builtin_amdgcn_readfirstlane(lim);
+}
+// Block tables through scalar loads: a vector load's wait would be one for the copies in flight, too.
+typedef const __attribute__((address_space(4))) int* table_t;
+__device__ __forceinline__ table_t table_of(const Args& A, const Work& W) {
+  return (table_t)(uintptr_t)(A.bt + (size_t)W.table * A.bt_stride);
+}
+__device__ __forceinline__ int page_at(const Args& A, table_t btr, int at) {
   return min(max(btr[at], 0), A.num_pages - 1);
 }
 
@@ -83,8 +93,9 @@ __device__ __forceinline__ f32x4 get_row(const float* so, int pair, int piece) {
   return *reinterpret_cast<const f32x4*>(so + pair * HD + ((piece ^ pair) << 2));
 }
 
-__device__ __forceinline__ size_t part_at(const Args& A, const Work& W, int kvh, int pair) {
-  return ((size_t)(A.base[W.row0 + pair / A.G] + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
+// where a pair's result of this part belongs
+__device__ __forceinline__ long part_at(const Args& A, const Work& W, int kvh, int pair) {
+  return ((long)(A.base[W.row0 + pair / A.G] + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -105,7 +116,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
   const int r32 = lane & 31, hh = lane >> 5;
   const Share S = share_of(W, most_of(A, W, lane));
   const int pairs = W.n * A.G, mine = w * 32 + r32, pair = min(mine, pairs - 1), row = W.row0 + pair / A.G;
-  const int lim = min(A.ctx_lens[row], A.max_ctx);
+  const int lim = min(A.ctx_lens[row], A.max_ctx), least = least_of(lim);
   f32x16 o[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -114,48 +125,55 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
   float m = -INFINITY, l = 0.f;
   if (S.first < S.end) {
     const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
-    const int* btr = A.bt + (size_t)W.table * A.bt_stride;
+    const table_t btr = table_of(A, W);
+    // an instruction takes four rows of 256 bytes; rows past the last key (whatever they hold) are that key's again
     constexpr int CP = 16 / NW;
     const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds)) + w * 1024;
     const int cr = 4 * w + (lane >> 4), cp = lane & 15;
-    // an instruction takes four rows of 256 bytes; rows past the last key (whatever they hold) are that key's again
-    auto copy = [&](const bf16* pool, int kt, int page, unsigned dst, bool is_v) {
+    unsigned koff[CP], voff[CP];
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const int r = cr + 4 * NW * i;
+      koff[i] = r * (HD * 2) + ((cp ^ (r & 15)) << 4);
+      voff[i] = r * (HD * 2) + ((cp ^ (4 * (r & 3))) << 4);
+    }
+    auto copy = [&](const bf16* pool, int kt, int page, unsigned dst, const unsigned (&off)[CP]) {
       const bf16* from = pool + (size_t)page * page_sz + head_off;
       const int top = S.last - kt * PAGE;
+      if (top >= PAGE - 1) {
 #pragma unroll
-      for (int i = 0; i < CP; ++i) {
-        const int r = cr + 4 * NW * i;
-        ldsp::dma_lds16(from, min(r, top) * (HD * 2) + ((cp ^ (is_v ? 4 * (r & 3) : r & 15)) << 4), dst + i * NW * 1024);
+        for (int i = 0; i < CP; ++i) ldsp::dma_lds16(from, off[i], dst + i * NW * 1024);
+      } else {
+#pragma unroll
+        for (int i = 0; i < CP; ++i)
+          ldsp::dma_lds16(from, off[i] - max(cr + 4 * NW * i - top, 0) * (HD * 2), dst + i * NW * 1024);
       }
     };
-    auto copy_k = [&](int kt, int page) { copy(A.kc, kt, page, l0 + (kt & 1) * (PG * 2), false); };
-    auto copy_v = [&](int kt, int page) { copy(A.vc, kt, page, l0 + (2 + (kt & 1)) * (PG * 2), true); };
+    auto copy_k = [&](int kt, int page) { copy(A.kc, kt, page, l0 + (kt & 1) * (PG * 2), koff); };
+    auto copy_v = [&](int kt, int page) { copy(A.vc, kt, page, l0 + (2 + (kt & 1)) * (PG * 2), voff); };
     auto page_of = [&](int kt) { return page_at(A, btr, min(kt, S.end - 1)); };
     int p0 = page_of(S.first), p1 = page_of(S.first + 1);   // pages kt and kt + 1
     bf16x8 qf[8];
     load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
     copy_k(S.first, p0);
 
+    // places of this lane in a stage: K rows kperm(r32) (and 32 further), V as read_v8 takes it
     const int krow = kperm(r32), L = lane & 15;
-    const bf16* kl = lds + krow * HD;
-    const bf16* vl = lds + 2 * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1);
-    const int vp = 2 * ((lane >> 4) & 1) + ((L >> 1) & 1);
-    auto read_k = [&](int st, int kh, int s) {
-      return *reinterpret_cast<const bf16x8*>(kl + st * PG + 32 * kh * HD + (((2 * s + hh) ^ (krow & 15)) << 3));
-    };
-    // V^T of numbers 32 db + r32, keys 32 kh + 16 s2 + 8 hh + 0 .. 7
-    auto read_v = [&](int st, int db, int kh, int s2) {
-      return read_v8(vl + st * PG + (32 * kh + 16 * s2) * HD + ((((db ^ (L >> 2)) << 2) | vp) << 3));
-    };
+    int kat[8], vat[4];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) kat[s] = (S.first & 1) * PG + krow * HD + (((2 * s + hh) ^ (krow & 15)) << 3);
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+      vat[db] = (2 + (S.first & 1)) * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1) +
+                ((((db ^ (L >> 2)) << 2) | (2 * ((lane >> 4) & 1) + ((L >> 1) & 1))) << 3);
     f32x16 sc[2];
     bf16x8 pf[2][2];   // P^T of the page before
-    // O^T += V^T . P^T of page `of` in eight pairs of products; LDS reads go out a pair ahead, and between them runs `work`
-    auto second_product = [&](int of, auto&& work) {
-      const int st = of & 1;
+    // O^T += V^T . P^T of the page before in eight pairs of products; LDS reads go out a pair ahead, and between them runs `work`
+    auto second_product = [&](auto&& work) {
       bf16x8 vf[2][2];
-      auto read_v2 = [&](int j) {
+      auto read_v2 = [&](int j) {   // numbers 32 (j / 2) .., keys 32 (j & 1) + 16 i ..
 #pragma unroll
-        for (int i = 0; i < 2; ++i) vf[j & 1][i] = read_v(st, j >> 1, j & 1, i);
+        for (int i = 0; i < 2; ++i) vf[j & 1][i] = read_v8(lds + vat[j >> 1] + (32 * (j & 1) + 16 * i) * HD);
       };
       read_v2(0);
 #pragma unroll
@@ -168,8 +186,11 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         work(j);
         __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int db = 0; db < 4; ++db) vat[db] ^= PG;
     };
-    for (int kt = S.first; kt < S.end; ++kt) {
+    // S^T = K . Q^T of page kt, two halves of 32 keys; the copies of its V and of the next K go out first
+    auto first_product = [&](int kt) {
       // K of this page and V of the one before have landed; every wave is past the last page's K and the V before it
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
@@ -177,37 +198,38 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       if (kt + 1 < S.end) copy_k(kt + 1, p1);
       p0 = p1;
       p1 = page_of(kt + 2);
-      {
-        bf16x8 kf[2][2];
-        auto read_k2 = [&](int s) {
+      bf16x8 kf[2][2];
+      auto read_k2 = [&](int s) {
 #pragma unroll
-          for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = read_k(kt & 1, kh, s);
-        };
-        read_k2(0);
+        for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = *reinterpret_cast<const bf16x8*>(lds + kat[s] + 32 * kh * HD);
+      };
+      read_k2(0);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        if (s < 7) read_k2(s + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kh][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          if (s < 7) read_k2(s + 1);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int kh = 0; kh < 2; ++kh)
-            sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s & 1][kh], qf[s], sc[kh], 0, 0, 0);
-        }
+          sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s & 1][kh], qf[s], s == 0 ? f32x16{} : sc[kh], 0, 0, 0);
       }
-      // Keys of register rr of half kh: 16 (rr >> 3) + 8 hh + (rr & 7).  O and l are rescaled only when some row's maximum grew
-      // by more than 2^8 (wave-uniform): until then weights stay below 2^8, as exact in bf16 as below 1.
-      constexpr float RESCALE_THR = 8.f;
-      const int k0 = kt * PAGE;
-      if (__any(k0 + PAGE > lim)) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s) kat[s] ^= PG;
+      // Keys of register rr of half kh: 16 (rr >> 3) + 8 hh + (rr & 7)
+      const int left = lim - kt * PAGE - 8 * hh;
+      if (kt * PAGE + PAGE > least) {
+        asm volatile("");   // (a branch, not selects on every page)
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
           for (int rr = 0; rr < 16; ++rr)
-            if (k0 + 32 * kh + 16 * (rr >> 3) + 8 * hh + (rr & 7) >= lim) sc[kh][rr] = -INFINITY;
+            if (32 * kh + 16 * (rr >> 3) + (rr & 7) >= left) sc[kh][rr] = -INFINITY;
       }
+    };
+    float alpha, mc, ps;
+    // The maxima.  O and l are rescaled only when some row's grew by more than 2^8 (wave-uniform): until then weights stay
+    // below 2^8, as exact in bf16 as below 1.
+    auto maxima = [&] {
+      constexpr float RESCALE_THR = 8.f;
       float mx = -INFINITY;
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh)
@@ -215,56 +237,73 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         for (int rr = 0; rr < 16; ++rr) mx = fmaxf(mx, sc[kh][rr]);
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const bool rescale = __any((mx - m) * A.scale_log2 > RESCALE_THR);
-      float alpha = 1.f;
       if (rescale) {
         const float mn = fmaxf(m, mx);
         alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * A.scale_log2);   // (no key yet: -inf both)
         m = mn;
         l *= alpha;
       }
-      const float mc = m == -INFINITY ? 0.f : m * A.scale_log2;
-      float ps = 0.f;
-      bf16x8 pn[2][2];
-      auto exps = [&](int j) {
+      mc = m == -INFINITY ? 0.f : m * A.scale_log2;
+      ps = 0.f;
+      int again = __builtin_amdgcn_readfirstlane(rescale);
+      asm volatile("" : "+s"(again));   // (one copy of what follows, not one for each side of the branch)
+      return again;
+    };
+    unsigned pn[4][4];   // this page's P^T
+    auto exps = [&](int j) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int kh = j >> 2, rr = (j & 3) * 4 + e;
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr], A.scale_log2, -mc));
-          ps += p;
-          pn[kh][rr >> 3][rr & 7] = f2bf(p);
-        }
-      };
-      if (kt > S.first) {
-        second_product(kt - 1, exps);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) exps(j);
+      for (int e = 0; e < 4; e += 2) {
+        const int kh = j >> 2, rr = (j & 3) * 4 + e;
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr], A.scale_log2, -mc));
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr + 1], A.scale_log2, -mc));
+        ps += x + y;
+        const bf16x2 xy = {f2bf(x), f2bf(y)};
+        pn[2 * kh + (rr >> 3)][(rr & 7) / 2] = __builtin_bit_cast(unsigned, xy);
+        // (formed here, between the products, not where they are used)
+        asm volatile("" : "+v"(pn[2 * kh + (rr >> 3)][(rr & 7) / 2]), "+v"(ps));
       }
+    };
+    auto take = [&] {
       l += ps;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        pf[i >> 1][i & 1] = __builtin_bit_cast(bf16x8, u32x4{pn[i][0], pn[i][1], pn[i][2], pn[i][3]});
+      }
+    };
+    first_product(S.first);
+    maxima();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) exps(j);
+    take();
+    for (int kt = S.first + 1; kt < S.end; ++kt) {
+      first_product(kt);
+      const int rescale = maxima();
+      second_product(exps);
+      take();
       if (rescale) {   // (O has the page before by now, which the old maximum scaled)
 #pragma unroll
         for (int db = 0; db < 4; ++db) o[db] *= alpha;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pf[i >> 1][i & 1] = pn[i >> 1][i & 1];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    second_product(S.end - 1, [](int) {});
+    second_product([](int) {});
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
+  const bool any = S.first < S.end;   // (a part of no page has its maximum only)
+  const long to = mine < pairs ? part_at(A, W, kvh, mine) : -1;
+  if (hh == 0 && to >= 0) A.part_ml[to] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
+  if (!any) return;
   // the wavefront's rows to LDS and from there in whole rows
   float* so = reinterpret_cast<float*>(lds) + w * (32 * HD);
   put_rows(so, o, r32, hh);
-  if (hh == 0 && mine < pairs)
-    A.part_ml[part_at(A, W, kvh, mine)] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int p = 2 * i + hh;
-    if (w * 32 + p < pairs)
-      *reinterpret_cast<f32x4*>(A.part_o + part_at(A, W, kvh, w * 32 + p) * HD + 4 * r32) = get_row(so, p, r32);
+    const long at = __shfl(to, 2 * i + hh, 64);
+    if (at >= 0) *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = get_row(so, 2 * i + hh, r32);
   }
 }
 
@@ -274,17 +313,16 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
 // meet at the end.
 constexpr int KT = 32;
 
-__device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, float2 (*sml)[ROWS], int tid, int w,
-                                         int lane) {
+__device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, int w, int lane) {
   bf16* lds = lds_all + w * (2 * KT * HD);   // K and V; O at the end
   const int r32 = lane & 31, hh = lane >> 5;
   const int pairs = W.n * A.G, pair = min(r32, pairs - 1), row = W.row0 + pair / A.G;
-  const int lim = min(A.ctx_lens[row], A.max_ctx);
+  const int lim = min(A.ctx_lens[row], A.max_ctx), least = least_of(lim);
   const Share S = share_of(W, most_of(A, W, lane));
   const int u0 = S.first * 2 + w, u1 = S.first < S.end ? S.last / KT + 1 : 0;   // units of 32 keys, this wavefront's every fourth
 
   const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
-  const int* btr = A.bt + (size_t)W.table * A.bt_stride;
+  const table_t btr = table_of(A, W);
   const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds));
   const int cr = lane >> 4, cp = lane & 15;
   auto copy = [&](const bf16* pool, int u, int page, bool is_v) {
@@ -339,11 +377,12 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
 #pragma unroll
         for (int s = 0; s < 8; ++s) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qf[s], sc, 0, 0, 0);
       }
-      const int k0 = u * KT;
-      if (__any(k0 + KT > lim)) {
+      const int left = lim - u * KT - 8 * hh;
+      if (u * KT + KT > least) {
+        asm volatile("");
 #pragma unroll
         for (int rr = 0; rr < 16; ++rr)
-          if (k0 + 16 * (rr >> 3) + 8 * hh + (rr & 7) >= lim) sc[rr] = -INFINITY;
+          if (16 * (rr >> 3) + (rr & 7) >= left) sc[rr] = -INFINITY;
       }
       float mx = sc[0];
 #pragma unroll
@@ -386,42 +425,60 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     }
   }
   l += __shfl_xor(l, 32, 64);
+  const long to = r32 < pairs ? part_at(A, W, kvh, r32) : -1;
+  if (S.first >= S.end) {   // a part of no page has its maximum only
+    if (w == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  // the four meet: first their maxima and sums (where all wavefronts' copies have been), then O in their place
+  constexpr int EACH = ROWS * 32 / (NW * 64);   // 16-byte pieces of a thread
+  float2* sml = reinterpret_cast<float2*>(lds_all);
+  __syncthreads();
+  if (hh == 0) sml[w * ROWS + r32] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
+  __syncthreads();
+  float weight[EACH][NW], M[EACH], den[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    float2 ml[NW];
+    M[i] = -INFINITY;
+    den[i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      ml[x] = sml[x * ROWS + i * 8 + w * 2 + hh];
+      M[i] = fmaxf(M[i], ml[x].x);
+    }
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      weight[i][x] = ml[x].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[x].x - M[i]);
+      den[i] = fmaf(weight[i][x], ml[x].y, den[i]);
+    }
+  }
+  __syncthreads();
   put_rows(reinterpret_cast<float*>(lds), o, r32, hh);
-  if (hh == 0) sml[w][r32] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(lds_all);
 #pragma unroll
-  for (int i = 0; i < ROWS * 32 / (NW * 64); ++i) {
-    const int at = tid + i * NW * 64, p = at >> 5, piece = at & 31;
-    if (p >= pairs) break;
-    float M = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) M = fmaxf(M, sml[x][p].x);
+  for (int i = 0; i < EACH; ++i) {
+    const int p = i * 8 + w * 2 + hh;
+    const long at = __shfl(to, p, 64);
+    if (at < 0) continue;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    float den = 0.f;
 #pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      const float2 ml = sml[x][p];
-      const float e = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
-      sum += get_row(all + x * (KT * HD), p, piece) * e;
-      den = fmaf(e, ml.y, den);
-    }
-    const size_t to = part_at(A, W, kvh, p);
-    *reinterpret_cast<f32x4*>(A.part_o + to * HD + 4 * piece) = sum;
-    if (piece == 0) A.part_ml[to] = make_float2(M, den);
+    for (int x = 0; x < NW; ++x) sum += get_row(all + x * (KT * HD), p, r32) * weight[i][x];
+    *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = sum;
+    if (r32 == 0) A.part_ml[at] = make_float2(M[i], den[i]);
   }
 }
 
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(
     Args A, const Work* __restrict__ works) {
   __shared__ __attribute__((aligned(16))) bf16 lds[4 * PG];
-  __shared__ float2 sml[NW][ROWS];
   // heads first: with 8 kv heads an XCD has one of them, and its L2 that head's pages for all tiles
   const int b = blockIdx.x;
   const Work W = works[b / A.Hkv];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   if (W.n * A.G > ROWS) tile_role(A, W, b % A.Hkv, lds, w, lane);
-  else few_role(A, W, b % A.Hkv, lds, sml, tid, w, lane);
+  else few_role(A, W, b % A.Hkv, lds, w, lane);
 }
 
 // One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
@@ -488,9 +545,9 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* 
 #pragma unroll 8
     for (int j = 0; j < nj; ++j) {
       const float2 v = *reinterpret_cast<const float2*>(po + (size_t)(sub + WPP * (j0 + j)) * Hq * HD);
-      const float ec = __shfl(e, j, 64);
-      acc[0] = fmaf(ec, v.x, acc[0]);
-      acc[1] = fmaf(ec, v.y, acc[1]);
+      const float ec = __shfl(e, j, 64);   // 0: of no weight, and nothing written where it had no page
+      acc[0] = fmaf(ec, ec == 0.f ? 0.f : v.x, acc[0]);
+      acc[1] = fmaf(ec, ec == 0.f ? 0.f : v.y, acc[1]);
     }
   }
   den = wave_sum(den);
