@@ -31,13 +31,16 @@ __device__ __forceinline__ int kperm(int rho) {  // S^T row rho -> key within th
 
 constexpr int NW = 4, ROWS = 32;
 constexpr int PG = PAGE * HD;                    // numbers of a page's K (V)
+constexpr int KST = 3;                           // stages of K in a tile (V: two)
 
 struct Args {
   const bf16 *q, *kc, *vc;
   const int *bt, *ctx_lens, *base;
   float* part_o;
   float2* part_ml;
-  int ldq, num_pages, bt_stride, max_ctx, Hkv, G;
+  bf16* out;
+  int ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G;
+  int whole;             // every row has one part, which is its result
   float scale_log2;
 };
 
@@ -71,6 +74,11 @@ __device__ __forceinline__ int page_at(const Args& A, table_t btr, int at) {
   return min(max(btr[at], 0), A.num_pages - 1);
 }
 
+__device__ __forceinline__ float max_of_halves(float x) {   // of lanes i and i + 32
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
 // Q^T operand of a lane's (row, head) pair: k-step s covers numbers 16 s .. 16 s + 15, lane half hh has 8 hh .. 8 hh + 7
 __device__ __forceinline__ void load_q(const Args& A, int row, int head, int hh, bf16x8 (&qf)[8]) {
   const bf16* qp = A.q + (size_t)row * A.ldq + (size_t)head * HD + 8 * hh;
@@ -97,6 +105,71 @@ __device__ __forceinline__ f32x4 get_row(const float* so, int pair, int piece) {
 __device__ __forceinline__ long part_at(const Args& A, const Work& W, int kvh, int pair) {
   return ((long)(A.base[W.row0 + pair / A.G] + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
 }
+
+// One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
+// give 0 * inf = nan to rows of the tile that do not see the value.
+__device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const int* btr, int num_pages, size_t page_sz,
+                           size_t head_off, int ctx, float scale_log2, int lane, float (&acc)[2]) {
+  float m = -INFINITY, l = 0.f;
+  acc[0] = acc[1] = 0.f;
+  for (int k0 = 0; k0 < ctx; k0 += PAGE) {
+    const size_t page = (size_t)min(max(btr[k0 / PAGE], 0), num_pages - 1) * page_sz + head_off;
+    float s = -INFINITY;
+    if (k0 + lane < ctx) {
+      const bf16* kp = kc + page + (size_t)lane * HD;
+      s = 0.f;
+      for (int d = 0; d < HD; ++d) s = fmaf((float)kp[d], (float)qp[d], s);
+      s *= scale_log2;
+    }
+    const float mn = fmaxf(m, wave_max(s));
+    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    const float p = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);
+    m = mn;
+    l = fmaf(l, alpha, wave_sum(p));
+    acc[0] *= alpha;
+    acc[1] *= alpha;
+    const int n = min(PAGE, ctx - k0);
+    for (int j = 0; j < n; ++j) {
+      const float pj = __shfl(p, j, 64);
+      const bf16x2 v = *reinterpret_cast<const bf16x2*>(vc + page + (size_t)j * HD + 2 * lane);
+      acc[0] = fmaf(pj, (float)v[0], acc[0]);
+      acc[1] = fmaf(pj, (float)v[1], acc[1]);
+    }
+  }
+  acc[0] /= l;
+  acc[1] /= l;
+}
+// the same for row r's head h, from the row's block table `btr`
+__device__ void exact_pair(const Args& A, const int* btr, int r, int h, int lane, float (&acc)[2]) {
+  exact_pair(A.q + (size_t)r * A.ldq + (size_t)h * HD, A.kc, A.vc, btr, A.num_pages, (size_t)A.Hkv * PG, (size_t)(h / A.G) * PG,
+             min(A.ctx_lens[r], A.max_ctx), A.scale_log2, lane, acc);
+}
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
+
+// Result of pair `pair` from its only part: lane r32 has numbers 4 r32 ..  A bit of `bad` says that it has to be done again.
+__device__ __forceinline__ bool put_result(const Args& A, const Work& W, int kvh, int pair, f32x4 sum, float den, int r32) {
+  const float by = den == 0.f ? 0.f : 1.f / den;   // (0: no key)
+  bf16x4 y;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = sum[i] * by;
+    bad |= not_finite(x);
+    y[i] = f2bf(x);
+  }
+  bf16* op = A.out + (size_t)(W.row0 + pair / A.G) * A.ldo + (size_t)(kvh * A.G + pair % A.G) * HD + 4 * r32;
+  *reinterpret_cast<bf16x4_u*>(op) = y;
+  return bad;
+}
+__device__ void put_exact(const Args& A, const Work& W, int kvh, int pair, int lane) {
+  const int r = W.row0 + pair / A.G, h = kvh * A.G + pair % A.G;
+  float acc[2];
+  exact_pair(A, A.bt + (size_t)W.table * A.bt_stride, r, h, lane, acc);
+  bf16* op = A.out + (size_t)r * A.ldo + (size_t)h * HD + 2 * lane;
+  op[0] = f2bf(acc[0]);
+  op[1] = f2bf(acc[1]);
+}
+
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds4_t;
@@ -149,23 +222,26 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
           ldsp::dma_lds16(from, off[i] - max(cr + 4 * NW * i - top, 0) * (HD * 2), dst + i * NW * 1024);
       }
     };
-    auto copy_k = [&](int kt, int page) { copy(A.kc, kt, page, l0 + (kt & 1) * (PG * 2), koff); };
-    auto copy_v = [&](int kt, int page) { copy(A.vc, kt, page, l0 + (2 + (kt & 1)) * (PG * 2), voff); };
+    auto copy_k = [&](int kt, int page, int stage) { copy(A.kc, kt, page, l0 + stage * (PG * 2), koff); };
+    auto copy_v = [&](int kt, int page) { copy(A.vc, kt, page, l0 + (KST + ((kt - S.first) & 1)) * (PG * 2), voff); };
     auto page_of = [&](int kt) { return page_at(A, btr, min(kt, S.end - 1)); };
-    int p0 = page_of(S.first), p1 = page_of(S.first + 1);   // pages kt and kt + 1
+    int p0 = page_of(S.first), p1 = page_of(S.first + 1), p2 = page_of(S.first + 2);   // pages kt, kt + 1, kt + 2
+    int kst = 0, flip = PG * 2;                                                        // stage of K; from this of V to the other
     bf16x8 qf[8];
     load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
-    copy_k(S.first, p0);
+    copy_k(S.first, p0, 0);
+    if (S.first + 1 < S.end) copy_k(S.first + 1, p1, 1);
 
     // places of this lane in a stage: K rows kperm(r32) (and 32 further), V as read_v8 takes it
     const int krow = kperm(r32), L = lane & 15;
-    int kat[8], vat[4];
+    int kat[8], vat[4];   // (in bytes)
 #pragma unroll
-    for (int s = 0; s < 8; ++s) kat[s] = (S.first & 1) * PG + krow * HD + (((2 * s + hh) ^ (krow & 15)) << 3);
+    for (int s = 0; s < 8; ++s) kat[s] = (krow * HD + (((2 * s + hh) ^ (krow & 15)) << 3)) * 2;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
-      vat[db] = (2 + (S.first & 1)) * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1) +
-                ((((db ^ (L >> 2)) << 2) | (2 * ((lane >> 4) & 1) + ((L >> 1) & 1))) << 3);
+      vat[db] = (KST * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1) +
+                 ((((db ^ (L >> 2)) << 2) | (2 * ((lane >> 4) & 1) + ((L >> 1) & 1))) << 3)) * 2;
+    const char* at_lds = reinterpret_cast<const char*>(lds);
     f32x16 sc[2];
     bf16x8 pf[2][2];   // P^T of the page before
     // O^T += V^T . P^T of the page before in eight pairs of products; LDS reads go out a pair ahead, and between them runs `work`
@@ -173,7 +249,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       bf16x8 vf[2][2];
       auto read_v2 = [&](int j) {   // numbers 32 (j / 2) .., keys 32 (j & 1) + 16 i ..
 #pragma unroll
-        for (int i = 0; i < 2; ++i) vf[j & 1][i] = read_v8(lds + vat[j >> 1] + (32 * (j & 1) + 16 * i) * HD);
+        for (int i = 0; i < 2; ++i) vf[j & 1][i] = read_v8(reinterpret_cast<const bf16*>(at_lds + vat[j >> 1]) + (32 * (j & 1) + 16 * i) * HD);
       };
       read_v2(0);
 #pragma unroll
@@ -181,27 +257,32 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         if (j < 7) read_v2(j + 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
           o[j >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 1][i], pf[j & 1][i], o[j >> 1], 0, 0, 0);
-        work(j);
-        __builtin_amdgcn_sched_barrier(0);
+          work(2 * j + i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
 #pragma unroll
-      for (int db = 0; db < 4; ++db) vat[db] ^= PG;
+      for (int db = 0; db < 4; ++db) vat[db] += flip;
+      flip = -flip;
     };
     // S^T = K . Q^T of page kt, two halves of 32 keys; the copies of its V and of the next K go out first
     auto first_product = [&](int kt) {
       // K of this page and V of the one before have landed; every wave is past the last page's K and the V before it
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      // (behind them the next K's copies, where there is one)
+      if (kt + 1 < S.end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CP) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       copy_v(kt, p0);
-      if (kt + 1 < S.end) copy_k(kt + 1, p1);
+      if (kt + 2 < S.end) copy_k(kt + 2, p2, kst == 0 ? KST - 1 : kst - 1);
       p0 = p1;
-      p1 = page_of(kt + 2);
+      p1 = p2;
+      p2 = page_of(kt + 3);
       bf16x8 kf[2][2];
       auto read_k2 = [&](int s) {
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = *reinterpret_cast<const bf16x8*>(lds + kat[s] + 32 * kh * HD);
+        for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = *reinterpret_cast<const bf16x8*>(at_lds + (kat[s] + kst * (PG * 2)) + 32 * kh * HD * 2);
       };
       read_k2(0);
 #pragma unroll
@@ -212,8 +293,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         for (int kh = 0; kh < 2; ++kh)
           sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s & 1][kh], qf[s], s == 0 ? f32x16{} : sc[kh], 0, 0, 0);
       }
-#pragma unroll
-      for (int s = 0; s < 8; ++s) kat[s] ^= PG;
+      kst = kst == KST - 1 ? 0 : kst + 1;
       // Keys of register rr of half kh: 16 (rr >> 3) + 8 hh + (rr & 7)
       const int left = lim - kt * PAGE - 8 * hh;
       if (kt * PAGE + PAGE > least) {
@@ -230,12 +310,13 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     // below 2^8, as exact in bf16 as below 1.
     auto maxima = [&] {
       constexpr float RESCALE_THR = 8.f;
-      float mx = -INFINITY;
+      float mx = fmaxf(sc[0][0], sc[1][0]), my = fmaxf(sc[0][1], sc[1][1]);
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-        for (int rr = 0; rr < 16; ++rr) mx = fmaxf(mx, sc[kh][rr]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      for (int rr = 2; rr < 16; rr += 2) {
+        mx = fmaxf(fmaxf(mx, sc[0][rr]), sc[1][rr]);
+        my = fmaxf(fmaxf(my, sc[0][rr + 1]), sc[1][rr + 1]);
+      }
+      mx = max_of_halves(fmaxf(mx, my));
       const bool rescale = __any((mx - m) * A.scale_log2 > RESCALE_THR);
       if (rescale) {
         const float mn = fmaxf(m, mx);
@@ -250,18 +331,15 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       return again;
     };
     unsigned pn[4][4];   // this page's P^T
-    auto exps = [&](int j) {
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const int kh = j >> 2, rr = (j & 3) * 4 + e;
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr], A.scale_log2, -mc));
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr + 1], A.scale_log2, -mc));
-        ps += x + y;
-        const bf16x2 xy = {f2bf(x), f2bf(y)};
-        pn[2 * kh + (rr >> 3)][(rr & 7) / 2] = __builtin_bit_cast(unsigned, xy);
-        // (formed here, between the products, not where they are used)
-        asm volatile("" : "+v"(pn[2 * kh + (rr >> 3)][(rr & 7) / 2]), "+v"(ps));
-      }
+    auto exps = [&](int j) {   // two of 32
+      const int kh = j >> 3, rr = (j & 7) * 2;
+      const float x = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr], A.scale_log2, -mc));
+      const float y = __builtin_amdgcn_exp2f(fmaf(sc[kh][rr + 1], A.scale_log2, -mc));
+      const bf16x2 xy = {f2bf(x), f2bf(y)}, ones = {(bf16)1.f, (bf16)1.f};
+      ps = __builtin_amdgcn_fdot2_f32_bf16(xy, ones, ps, false);   // (of the weights as they go into the product)
+      pn[2 * kh + (rr >> 3)][(rr & 7) / 2] = __builtin_bit_cast(unsigned, xy);
+      // (formed here, between the products, not where they are used)
+      asm volatile("" : "+v"(pn[2 * kh + (rr >> 3)][(rr & 7) / 2]), "+v"(ps));
     };
     auto take = [&] {
       l += ps;
@@ -274,7 +352,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     first_product(S.first);
     maxima();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) exps(j);
+    for (int j = 0; j < 16; ++j) exps(j);
     take();
     for (int kt = S.first + 1; kt < S.end; ++kt) {
       first_product(kt);
@@ -292,12 +370,26 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
-  const bool any = S.first < S.end;   // (a part of no page has its maximum only)
+  float* so = reinterpret_cast<float*>(lds) + w * (32 * HD);   // the wavefront's rows, to be written whole
+  if (A.whole) {
+    put_rows(so, o, r32, hh);
+    __builtin_amdgcn_wave_barrier();
+    unsigned bad = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int p = 2 * i + hh;
+      const float den = __shfl(l, p, 64);
+      if (w * 32 + p < pairs) bad |= (unsigned)put_result(A, W, kvh, w * 32 + p, get_row(so, p, r32), den, r32) << i;
+    }
+    if (__any(bad)) {
+      for (int p = 0; p < 32; ++p)
+        if ((__ballot(bad >> (p / 2) & 1) >> (32 * (p & 1))) & 0xffffffffull) put_exact(A, W, kvh, w * 32 + p, lane);
+    }
+    return;
+  }
   const long to = mine < pairs ? part_at(A, W, kvh, mine) : -1;
   if (hh == 0 && to >= 0) A.part_ml[to] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
-  if (!any) return;
-  // the wavefront's rows to LDS and from there in whole rows
-  float* so = reinterpret_cast<float*>(lds) + w * (32 * HD);
+  if (S.first >= S.end) return;   // (a part of no page has its maximum only)
   put_rows(so, o, r32, hh);
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -387,7 +479,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
       float mx = sc[0];
 #pragma unroll
       for (int rr = 1; rr < 16; ++rr) mx = fmaxf(mx, sc[rr]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      mx = max_of_halves(mx);
       const float mn = fmaxf(m, mx);
       const float ms = mn == -INFINITY ? 0.f : mn * A.scale_log2;    // no key yet: weights 0
       const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * A.scale_log2);
@@ -425,8 +517,8 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     }
   }
   l += __shfl_xor(l, 32, 64);
-  const long to = r32 < pairs ? part_at(A, W, kvh, r32) : -1;
-  if (S.first >= S.end) {   // a part of no page has its maximum only
+  const long to = r32 >= pairs ? -1 : A.whole ? 0 : part_at(A, W, kvh, r32);
+  if (!A.whole && S.first >= S.end) {   // a part of no page has its maximum only
     if (w == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(-INFINITY, 0.f);
     return;
   }
@@ -444,7 +536,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     den[i] = 0.f;
 #pragma unroll
     for (int x = 0; x < NW; ++x) {
-      ml[x] = sml[x * ROWS + i * 8 + w * 2 + hh];
+      ml[x] = sml[x * ROWS + 2 * (NW * i + w) + hh];
       M[i] = fmaxf(M[i], ml[x].x);
     }
 #pragma unroll
@@ -457,147 +549,143 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
   put_rows(reinterpret_cast<float*>(lds), o, r32, hh);
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(lds_all);
+  unsigned bad = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int p = i * 8 + w * 2 + hh;
+    const int p = 2 * (NW * i + w) + hh;
     const long at = __shfl(to, p, 64);
     if (at < 0) continue;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NW; ++x) sum += get_row(all + x * (KT * HD), p, r32) * weight[i][x];
+    if (A.whole) {
+      bad |= (unsigned)put_result(A, W, kvh, p, sum, den[i], r32) << i;
+      continue;
+    }
     *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = sum;
     if (r32 == 0) A.part_ml[at] = make_float2(M[i], den[i]);
+  }
+  if (__any(bad)) {
+    for (int i = 0; i < 2 * EACH; ++i)
+      if ((__ballot(bad >> (i / 2) & 1) >> (32 * (i & 1))) & 0xffffffffull)
+        put_exact(A, W, kvh, 2 * (NW * (i / 2) + w) + (i & 1), lane);
   }
 }
 
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(
     Args A, const Work* __restrict__ works) {
-  __shared__ __attribute__((aligned(16))) bf16 lds[4 * PG];
+  static_assert(NW * 2 * KT <= (KST + 2) * PAGE, "few_role in the LDS of tile_role");
+  __shared__ __attribute__((aligned(16))) bf16 lds[(KST + 2) * PG];
   // heads first: with 8 kv heads an XCD has one of them, and its L2 that head's pages for all tiles
   const int b = blockIdx.x;
   const Work W = works[b / A.Hkv];
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (W.n * A.G > ROWS) tile_role(A, W, b % A.Hkv, lds, w, lane);
   else few_role(A, W, b % A.Hkv, lds, w, lane);
 }
 
-// One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
-// give 0 * inf = nan to rows of the tile that do not see the value.
-__device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const int* btr, int num_pages, size_t page_sz,
-                           size_t head_off, int ctx, float scale_log2, int lane, float (&acc)[2]) {
-  float m = -INFINITY, l = 0.f;
-  acc[0] = acc[1] = 0.f;
-  for (int k0 = 0; k0 < ctx; k0 += PAGE) {
-    const size_t page = (size_t)min(max(btr[k0 / PAGE], 0), num_pages - 1) * page_sz + head_off;
-    float s = -INFINITY;
-    if (k0 + lane < ctx) {
-      const bf16* kp = kc + page + (size_t)lane * HD;
-      s = 0.f;
-      for (int d = 0; d < HD; ++d) s = fmaf((float)kp[d], (float)qp[d], s);
-      s *= scale_log2;
-    }
-    const float mn = fmaxf(m, wave_max(s));
-    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-    const float p = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, alpha, wave_sum(p));
-    acc[0] *= alpha;
-    acc[1] *= alpha;
-    const int n = min(PAGE, ctx - k0);
-    for (int j = 0; j < n; ++j) {
-      const float pj = __shfl(p, j, 64);
-      const bf16x2 v = *reinterpret_cast<const bf16x2*>(vc + page + (size_t)j * HD + 2 * lane);
-      acc[0] = fmaf(pj, (float)v[0], acc[0]);
-      acc[1] = fmaf(pj, (float)v[1], acc[1]);
-    }
-  }
-  acc[0] /= l;
-  acc[1] /= l;
-}
-
-// The parts of a row: WPP wavefronts per (row, head), two numbers per lane.  Many parts go to four wavefronts, which meet in
-// LDS: a wavefront has eight loads in flight.
-template <int WPP>
-__global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* __restrict__ tables, int R, bf16* __restrict__ out,
-                                                             int ldo) {
-  __shared__ float2 meet[4][64];
-  __shared__ float meet_den[4];
-  const int Hq = A.Hkv * A.G, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i = blockIdx.x * (4 / WPP) + w / WPP, sub = w % WPP;
-  if (i >= R * Hq) return;    // (WPP 4: the whole workgroup)
-  const int r = i / Hq, h = i % Hq;
-  const int b0 = A.base[r], n = A.base[r + 1] - b0;
+// The parts of a (row, head) pair: GROUPS half wavefronts, four numbers per lane, each with every GROUPS-th part.  A group has
+// the statistics and outputs of eight parts in flight together, what they weigh is known when they have come; groups meet in LDS.
+template <int GROUPS>
+__global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* __restrict__ tables, int R, int even) {
+  const int Hq = A.Hkv * A.G, lane = threadIdx.x & 63, r32 = lane & 31, g = GROUPS == 1 ? 0 : threadIdx.x >> 5;
+  const int pair0 = GROUPS == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, pair = min(pair0, R * Hq - 1);
+  const int r = pair / Hq, h = pair % Hq;
+  const int b0 = even ? r * even : A.base[r], n = even ? even : A.base[r + 1] - b0;
   const float2* ml = A.part_ml + (size_t)b0 * Hq + h;
-  const float* po = A.part_o + ((size_t)b0 * Hq + h) * HD + 2 * lane;
-  float M = -INFINITY;
-  for (int c = lane; c < n; c += 64) M = fmaxf(M, ml[(size_t)c * Hq].x);
-  M = wave_max(M);
-  float acc[2] = {0.f, 0.f}, den = 0.f;
-  for (int j0 = 0; sub + WPP * j0 < n; j0 += 64) {   // this wavefront's parts: sub + WPP j
-    const int c = sub + WPP * (j0 + lane);
-    float e = 0.f;
-    if (c < n) {
-      const float2 x = ml[(size_t)c * Hq];
-      e = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - M);
-      den = fmaf(e, x.y, den);
-    }
-    const int nj = min(64, (n - sub - WPP * j0 + WPP - 1) / WPP);
-#pragma unroll 8
-    for (int j = 0; j < nj; ++j) {
-      const float2 v = *reinterpret_cast<const float2*>(po + (size_t)(sub + WPP * (j0 + j)) * Hq * HD);
-      const float ec = __shfl(e, j, 64);   // 0: of no weight, and nothing written where it had no page
-      acc[0] = fmaf(ec, ec == 0.f ? 0.f : v.x, acc[0]);
-      acc[1] = fmaf(ec, ec == 0.f ? 0.f : v.y, acc[1]);
-    }
-  }
-  den = wave_sum(den);
-  if constexpr (WPP > 1) {
-    meet[w][lane] = make_float2(acc[0], acc[1]);
-    if (lane == 0) meet_den[w] = den;
-    __syncthreads();
-    if (w > 0) return;
-    acc[0] = acc[1] = den = 0.f;
+  const float* po = A.part_o + ((size_t)b0 * Hq + h) * HD + 4 * r32;
+  float M = -INFINITY, den = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = g; c0 < n; c0 += 8 * GROUPS) {
+    float2 st[8];
+    f32x4 o[8];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float2 v = meet[x][lane];
-      acc[0] += v.x;
-      acc[1] += v.y;
-      den += meet_den[x];
+    for (int j = 0; j < 8; ++j) {
+      const size_t c = (size_t)min(c0 + j * GROUPS, n - 1) * Hq;
+      st[j] = ml[c];
+      o[j] = *reinterpret_cast<const f32x4*>(po + c * HD);
+    }
+    float m = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = c0 + j * GROUPS < n ? fmaxf(m, st[j].x) : m;
+    const float alpha = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
+    M = m;
+    den *= alpha;
+    acc *= alpha;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (c0 + j * GROUPS >= n) break;
+      const float e = st[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[j].x - m);
+      den = fmaf(e, st[j].y, den);
+      // (of no weight: nothing may be written there)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = e == 0.f ? acc[i] : fmaf(e, o[j][i], acc[i]);
     }
   }
-  if (M == -INFINITY && !(den != den)) {
-    acc[0] = acc[1] = 0.f;    // no key
-  } else {
-    acc[0] /= den;
-    acc[1] /= den;
-    if (__any(!(fabsf(acc[0]) < INFINITY) || !(fabsf(acc[1]) < INFINITY)))
-      exact_pair(A.q + (size_t)r * A.ldq + (size_t)h * HD, A.kc, A.vc, A.bt + (size_t)tables[r] * A.bt_stride, A.num_pages,
-                 (size_t)A.Hkv * PG, (size_t)(h / A.G) * PG, min(A.ctx_lens[r], A.max_ctx), A.scale_log2, lane, acc);
+  if constexpr (GROUPS > 1) {
+    __shared__ f32x4 so[GROUPS][32];
+    __shared__ float2 sml[GROUPS];
+    so[g][r32] = acc;
+    if (r32 == 0) sml[g] = make_float2(M, den);
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < GROUPS; ++x) M = fmaxf(M, sml[x].x);
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    den = 0.f;
+#pragma unroll
+    for (int x = 0; x < GROUPS; ++x) {
+      const float2 s = sml[x];
+      const float e = s.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.x - M);
+      den = fmaf(e, s.y, den);
+      acc += so[x][r32] * e;
+    }
   }
-  bf16* op = out + (size_t)r * ldo + (size_t)h * HD + 2 * lane;
-  op[0] = f2bf(acc[0]);
-  op[1] = f2bf(acc[1]);
+  const float by = den == 0.f ? 0.f : 1.f / den;   // (0: no key)
+  bf16x4 y;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = acc[i] * by;
+    bad |= not_finite(x);
+    y[i] = f2bf(x);
+  }
+  if (pair0 < R * Hq && (GROUPS == 1 || g == 0))
+    *reinterpret_cast<bf16x4_u*>(A.out + (size_t)r * A.ldo + (size_t)h * HD + 4 * r32) = y;
+  const unsigned long long again = __ballot(bad);
+  if (again) {
+    for (int x = 0; x < (GROUPS == 1 ? 2 : 1); ++x) {
+      if (!(again >> (32 * x) & 0xffffffffull)) continue;
+      const int rx = __shfl(r, 32 * x, 64), hx = __shfl(h, 32 * x, 64);
+      float two[2];
+      exact_pair(A, A.bt + (size_t)tables[rx] * A.bt_stride, rx, hx, lane, two);
+      bf16* op = A.out + (size_t)rx * A.ldo + (size_t)hx * HD + 2 * lane;
+      op[0] = f2bf(two[0]);
+      op[1] = f2bf(two[1]);
+    }
+  }
 }
 
 }  // namespace
 
-// works: int32 [n_works, 8] (Work); base: int32 [R + 1], the parts of the rows before; tables: int32 [R], the rows' block
+// works: int32 [n_works, 8] (Work); base: int32 [R + 1], the parts of the rows before (even: every row has so many, or 0); tables: int32 [R], the rows' block
 // tables; part_o, part_ml: base[R] * Hq * (128 | 2) floats.  Every part of every row belongs to one work.
 P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int num_pages,
                                  const int* block_tables, int bt_stride, const int* ctx_lens, int max_ctx, const int* works,
-                                 int n_works, const int* base, const int* tables, int R, int parts, int Hq, int Hkv,
+                                 int n_works, const int* base, const int* tables, int R, int parts, int even, int Hq, int Hkv,
                                  int head_dim, float scale, void* out, int ldo, float* part_o, float* part_ml, hipStream_t stream) {
   if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0) return (int)hipErrorInvalidValue;
   const float sl2 = scale * 1.4426950408889634f;
   const int G = Hq / Hkv;
-  const bool many = parts > 8 * R;
   const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, base, part_o,
-                  (float2*)part_ml, ldq, num_pages, bt_stride, max_ctx, Hkv, G, sl2};
+                  (float2*)part_ml, (bf16*)out, ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G, parts == R, sl2};
   hipLaunchKernelGGL(prefix_attn_kernel, dim3(n_works * Hkv), dim3(NW * 64), 0, stream, A, (const Work*)works);
   if (int e = (int)hipGetLastError()) return e;
-  if (many)
-    hipLaunchKernelGGL(prefix_combine_kernel<4>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R, (bf16*)out, ldo);
+  if (parts == R) return 0;
+  if (parts > 8 * R)
+    hipLaunchKernelGGL(prefix_combine_kernel<8>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R, even);
   else
-    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 3) / 4), dim3(256), 0, stream, A, tables, R, (bf16*)out, ldo);
+    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 7) / 8), dim3(256), 0, stream, A, tables, R, even);
   P2P_CHECK_LAUNCH();
 }

@@ -38,7 +38,7 @@ _SIGS = {
                             c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int,
                             c_void_p, c_void_p, c_void_p],
     "p2p_prefix_attention": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
-                             c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p,
+                             c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p,
                              c_void_p, c_void_p],
     "p2p_copy_pages": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
                        c_void_p],
@@ -311,11 +311,12 @@ def stream_ptr(device=None) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def device_of(t):
-    """A context in which t's device is the current one (a launch on a stream of another device is an error)."""
-    if t.device.index in (None, torch.cuda.current_device()):
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+_HERE = contextlib.nullcontext()
+
+
+def device_of(index: int):
+    """A context in which the device is the current one (a launch on a stream of another device is an error)."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def check(err: int, name: str):

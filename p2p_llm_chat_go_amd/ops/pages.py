@@ -15,21 +15,24 @@ from .attention import HEAD_DIM, PAGE
 
 
 def _caches(k: torch.Tensor, v: torch.Tensor, what: str):
-    for name, c in (("k", k), ("v", v)):
-        if c.dim() != 5 or c.shape[3:] != (PAGE, HEAD_DIM):
-            raise ValueError("%s: %s must be [layers, pages, kv heads, %d, %d], got %s"
-                             % (what, name, PAGE, HEAD_DIM, list(c.shape)))
-        if c.element_size() not in (1, 2, 4) or c.is_complex():
-            raise ValueError("%s: %s has numbers of type %s" % (what, name, c.dtype))
-        if c.stride(4) != 1 or c.stride(3) != HEAD_DIM or any(s * c.element_size() % 16 for s in c.stride()[:3]) or c.data_ptr() % 16:
-            raise ValueError("%s: the tokens of a page of %s must be contiguous and start at multiples of 16 bytes" % (what, name))
-    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+    """Strides in bytes between layers, pages and heads of k, then of v."""
+    shape, strides = k.shape, k.stride() + v.stride()
+    if len(shape) != 5 or v.dim() != 5 or shape[3] != PAGE or shape[4] != HEAD_DIM:
+        raise ValueError("%s: k and v must be [layers, pages, kv heads, %d, %d], got %s and %s"
+                         % (what, PAGE, HEAD_DIM, list(shape), list(v.shape)))
+    if shape != v.shape or k.dtype != v.dtype or k.device != v.device:
         raise ValueError("%s: k and v differ in shape, type or device" % what)
-
-
-def _strides(k: torch.Tensor, v: torch.Tensor):
     size = k.element_size()
-    return (ctypes.c_long * 6)(*(s * size for c in (k, v) for s in c.stride()[:3]))
+    if size not in (1, 2, 4) or k.dtype.is_complex:
+        raise ValueError("%s: k and v have numbers of type %s" % (what, k.dtype))
+    kl, kp, kh, kt, k1, vl, vp, vh, vt, v1 = strides
+    if k1 != 1 or v1 != 1 or kt != HEAD_DIM or vt != HEAD_DIM or (kl | kp | kh | vl | vp | vh) * size % 16 \
+            or (k.data_ptr() | v.data_ptr()) % 16:
+        raise ValueError("%s: the tokens of a page must be contiguous and start at multiples of 16 bytes" % what)
+    return _SIX(kl * size, kp * size, kh * size, vl * size, vp * size, vh * size)
+
+
+_SIX = ctypes.c_long * 6
 
 
 def _ints(x, what: str) -> array.array:
@@ -48,7 +51,7 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src, dst, tokens=None) -> None:
 
     src, dst, tokens: host numbers, as allocators give them.  tokens: how many of a page's tokens are copied (None: all); the
     others of the page stay.  A page is in dst once at most and then not in src (but ``src[i] == dst[i]`` is nothing to do)."""
-    _caches(k, v, "copy_pages")
+    strides = _caches(k, v, "copy_pages")
     src, dst = _ints(src, "src"), _ints(dst, "dst")
     tokens = array.array("i", [PAGE]) * len(src) if tokens is None else _ints(tokens, "tokens")
     if not len(src) == len(dst) == len(tokens):
@@ -72,9 +75,9 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src, dst, tokens=None) -> None:
             k[:, d, :, :n] = k[:, s, :, :n]
             v[:, d, :, :n] = v[:, s, :, :n]
         return
-    with _lib.device_of(k):
+    with _lib.device_of(k.get_device()):
         _lib.check(_lib.lib().p2p_copy_pages(
-            k.data_ptr(), v.data_ptr(), _strides(k, v), k.shape[0], k.shape[2], P, HEAD_DIM * k.element_size(),
+            k.data_ptr(), v.data_ptr(), strides, k.shape[0], k.shape[2], P, HEAD_DIM * k.element_size(),
             src.buffer_info()[0], dst.buffer_info()[0], tokens.buffer_info()[0], len(src), _lib.stream_ptr(k.device)),
             "copy_pages")
 
@@ -112,7 +115,7 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
     cos_sin: float32 [positions, 64, 2] (``models.config.rope_table``): keys that were rotated for position p are turned on to
     position n (bf16 caches); None: they stay as they are, as for sequences that go on counting positions.  Entries of the
     tables that are no pages are skipped."""
-    _caches(k, v, "compact_pages")
+    strides = _caches(k, v, "compact_pages")
     def need(ok, why):
         if not ok:
             raise ValueError("compact_pages: " + why)
@@ -142,9 +145,9 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
         return new
     if k.numel() == 0 or most == 0:
         return new.copy_((keep & (torch.arange(keep.shape[1], device=k.device) < lens[:, None].clamp(max=most))).sum(1))
-    with _lib.device_of(k):
+    with _lib.device_of(k.get_device()):
         _lib.check(_lib.lib().p2p_compact_pages(
-            k.data_ptr(), v.data_ptr(), _strides(k, v), k.shape[0], k.shape[2], k.shape[1], HEAD_DIM * k.element_size(),
+            k.data_ptr(), v.data_ptr(), strides, k.shape[0], k.shape[2], k.shape[1], HEAD_DIM * k.element_size(),
             block_tables.data_ptr(), block_tables.stride(0), W, _lib.ptr(out_tables),
             0 if out_tables is None else out_tables.stride(0), lens.data_ptr(), keep.data_ptr(), keep.stride(0), keep.shape[1],
             B, _lib.ptr(cos_sin), new.data_ptr(), _lib.stream_ptr(k.device)), "compact_pages")

@@ -18,7 +18,9 @@ from . import _lib
 from .attention import HEAD_DIM, PAGE, paged_attention_ref
 
 import os
+ALONE=None
 TOTAL_SHARED=int(os.environ.get('TS','512')); TOTAL_OWN=int(os.environ.get('TO','1024'))
+SCALE = 1.0 / math.sqrt(HEAD_DIM)
 FEW, MANY = 32, 128    # (row, head) pairs of a workgroup, in the kernel's two roles
 
 
@@ -30,6 +32,7 @@ class PrefixPlan:
     n_kv: int
     max_ctx: int
     tables: int            # block tables it reads
+    even: int              # results of every row, where they are equally many (else 0)
     parts: int             # results of parts, over all rows
     works: torch.Tensor    # int32 [n, 8]
     base: torch.Tensor     # int32 [rows + 1]: parts of the rows before
@@ -73,6 +76,8 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
         """Rows a .. b - 1 as tiles."""
         tile = few if (b - a) * G <= FEW else many
         return [(i, min(tile, b - i)) for i in range(a, b, tile)]
+    if ALONE if ALONE is not None else False:
+        groups = [(r, 0) for r, _ in groups]
     shared, owned, r0 = [], [], 0        # (first row, rows, table, first page, last page + 1)
     for n, p in groups:
         r1 = r0 + n
@@ -98,7 +103,7 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
         for a, n, *_ in tiles:
             count[a:a + n] = [C] * n
     for a, n, t, p0, p1 in owned:
-        C = parts_of(len(owned), p1 - p0, TOTAL_OWN)
+        C = 1 if ALONE else parts_of(len(owned), p1 - p0, TOTAL_OWN)
         works += [(a, n, t, p0, p1, c, C, count[a]) for c in range(C)]
         count[a:a + n] = [count[a] + C] * n
     base = [0]
@@ -108,7 +113,7 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     flat = [x for w in works for x in w] + seqs + base
     flat = torch.tensor(flat, dtype=torch.int32).to(dev)
     n = 8 * len(works)
-    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, base[-1], flat[:n].view(-1, 8), flat[n + R:], flat[n:n + R])
+    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, count[0] if min(count) == max(count) else 0, base[-1], flat[:n].view(-1, 8), flat[n + R:], flat[n:n + R])
 
 
 def prefix_workspace(plan: PrefixPlan) -> tuple:
@@ -119,9 +124,33 @@ def prefix_workspace(plan: PrefixPlan) -> tuple:
             torch.empty(plan.parts * plan.n_heads * 2, device=dev, dtype=torch.float32))
 
 
-def _check(ok: bool, why: str):
-    if not ok:
-        raise ValueError("prefix_attention: " + why)
+def _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale):
+    """Says which of prefix_attention's conditions does not hold."""
+    R, n_heads, n_kv, width = plan.rows, plan.n_heads, plan.n_kv, plan.n_heads * HEAD_DIM
+    def need(ok, why):
+        if not ok:
+            raise ValueError("prefix_attention: " + why)
+    need(q.dim() == 2 and q.dtype == torch.bfloat16 and q.shape[0] >= R and q.shape[1] == width and q.stride(1) == 1,
+         "q must be bf16 [%d or more, %d], rows contiguous" % (R, width))
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        need(c.dim() == 4 and c.shape[1:] == (n_kv, PAGE, HEAD_DIM) and c.dtype == torch.bfloat16 and c.is_contiguous()
+             and c.shape[0] > 0 and c.data_ptr() % 16 == 0,
+             "%s must be bf16 [pages, %d, %d, %d], contiguous from a multiple of 16 bytes" % (name, n_kv, PAGE, HEAD_DIM))
+    need(k_cache.shape == v_cache.shape, "k_cache and v_cache differ in shape")
+    need(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
+         and block_tables.shape[0] >= plan.tables and block_tables.shape[1] * PAGE >= plan.max_ctx,
+         "block_tables must be int32 [%d or more, pages of %d tokens]" % (plan.tables, plan.max_ctx))
+    need(ctx_lens.dim() == 1 and ctx_lens.dtype == torch.int32 and ctx_lens.shape[0] >= R and ctx_lens.stride(0) == 1,
+         "ctx_lens must be int32 [%d or more]" % R)
+    need(0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
+    need(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width and out.stride(1) == 1,
+         "out must be bf16 [%d or more, %d], rows contiguous" % (R, width))
+    need(all(t.device == q.device for t in (k_cache, v_cache, block_tables, ctx_lens, plan.works, out) + workspace),
+         "tensors and plan must be on one device")
+    need(not workspace or all(w.dtype == torch.float32 and w.is_contiguous() for w in workspace), "workspace is not this plan's")
+    need(not workspace or (workspace[0].numel() >= plan.parts * width and workspace[1].numel() >= plan.parts * n_heads * 2),
+         "workspace is not this plan's")
+    raise AssertionError("prefix_attention: the two forms of its conditions differ")
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -134,42 +163,48 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     tables hold pages of the cache; others read page 0 or the last one."""
     R, n_heads, n_kv = plan.rows, plan.n_heads, plan.n_kv
     width = n_heads * HEAD_DIM
-    _check(q.dim() == 2 and q.dtype == torch.bfloat16 and q.shape[0] >= R and q.shape[1] == width
-           and (q.stride(1) == 1 or width == 1), "q must be bf16 [%d or more, %d], rows contiguous" % (R, width))
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _check(c.dim() == 4 and c.shape[1:] == (n_kv, PAGE, HEAD_DIM) and c.dtype == torch.bfloat16 and c.is_contiguous()
-               and c.shape[0] > 0, "%s must be bf16 [pages, %d, %d, %d], contiguous" % (name, n_kv, PAGE, HEAD_DIM))
-    _check(k_cache.shape == v_cache.shape, "k_cache and v_cache differ in shape")
-    _check(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
-           and block_tables.shape[0] >= plan.tables and block_tables.shape[1] * PAGE >= plan.max_ctx,
-           "block_tables must be int32 [%d or more, pages of %d tokens]" % (plan.tables, plan.max_ctx))
-    _check(ctx_lens.dim() == 1 and ctx_lens.dtype == torch.int32 and ctx_lens.shape[0] >= R and ctx_lens.stride(0) == 1,
-           "ctx_lens must be int32 [%d or more]" % R)
     if scale is None:
-        scale = 1.0 / math.sqrt(HEAD_DIM)
-    _check(0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
+        scale = SCALE
     if out is None:
-        out = torch.empty(q.shape[0], width, device=q.device, dtype=q.dtype)
-    _check(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width
-           and out.stride(1) == 1, "out must be bf16 [%d or more, %d], rows contiguous" % (R, width))
-    given = (q, k_cache, v_cache, block_tables, ctx_lens, plan.works, out) + tuple(workspace or ())
-    _check(all(t.device == q.device for t in given), "tensors and plan must be on one device")
-    if q.device.type != "cuda":
+        out = torch.empty(q.shape[0], width, device=q.device, dtype=torch.bfloat16)
+    dev = q.get_device()     # (-1: CPU)
+    if workspace is None:
+        workspace = prefix_workspace(plan) if dev >= 0 and plan.works.get_device() == dev else ()
+    works = plan.works
+    try:
+        Rq, wq = q.shape
+        Ro, wo = out.shape
+        tables, pages = block_tables.shape
+        rows, = ctx_lens.shape
+        P, h, t, d = shape = k_cache.shape
+        ok = (Rq >= R and wq == wo == width and Ro >= R and tables >= plan.tables and pages * PAGE >= plan.max_ctx and rows >= R
+              and shape == v_cache.shape and h == n_kv and t == PAGE and d == HEAD_DIM and P > 0
+              and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16
+              and block_tables.dtype == ctx_lens.dtype == torch.int32
+              and q.stride(1) == out.stride(1) == block_tables.stride(1) == ctx_lens.stride(0) == 1
+              and k_cache.is_contiguous() and v_cache.is_contiguous() and 0 < scale < math.inf
+              and dev == out.get_device() == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
+              == ctx_lens.get_device() == works.get_device() and q.device.type == k_cache.device.type == ctx_lens.device.type)
+        kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+        if ok and dev >= 0:
+            po, pml = workspace
+            ok = ((kp | vp) % 16 == 0 and po.get_device() == pml.get_device() == dev and po.dtype == pml.dtype == torch.float32
+                  and po.is_contiguous() and pml.is_contiguous() and po.numel() >= plan.parts * width
+                  and pml.numel() >= plan.parts * n_heads * 2)
+    except ValueError:       # another number of dimensions
+        ok = False
+    if not ok:
+        _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, tuple(workspace), scale)
+    if dev < 0:
         ctx = ctx_lens[:R].clamp(0, plan.max_ctx)
-        some = ctx > 0
         paged_attention_ref(q[:R], k_cache, v_cache, block_tables, plan.row_tables, ctx.clamp(min=1), n_heads, n_kv, scale,
                             out[:R])
-        out[:R] = torch.where(some[:, None], out[:R], 0)
+        out[:R] = torch.where((ctx > 0)[:, None], out[:R], 0)
         return out
-    if workspace is None:
-        workspace = prefix_workspace(plan)
-    po, pml = workspace
-    _check(po.dtype == pml.dtype == torch.float32 and po.is_contiguous() and pml.is_contiguous()
-           and po.numel() >= plan.parts * width and pml.numel() >= plan.parts * n_heads * 2, "workspace is not this plan's")
-    with _lib.device_of(q):
+    with _lib.device_of(dev):
         _lib.check(_lib.lib().p2p_prefix_attention(
-            q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_tables.data_ptr(),
-            block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx, plan.works.data_ptr(), plan.works.shape[0],
-            plan.base.data_ptr(), plan.row_tables.data_ptr(), R, plan.parts, n_heads, n_kv, HEAD_DIM, float(scale), out.data_ptr(),
-            out.stride(0), po.data_ptr(), pml.data_ptr(), _lib.stream_ptr(q.device)), "prefix_attention")
+            q.data_ptr(), q.stride(0), kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(),
+            plan.max_ctx, works.data_ptr(), works.shape[0], plan.base.data_ptr(), plan.row_tables.data_ptr(), R, plan.parts, plan.even,
+            n_heads, n_kv, HEAD_DIM, scale, out.data_ptr(), out.stride(0), po.data_ptr(), pml.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
     return out
