@@ -17,10 +17,9 @@ import torch
 from . import _lib
 from .attention import HEAD_DIM, PAGE, paged_attention_ref
 
-import os
-ALONE=None
-TOTAL_SHARED=int(os.environ.get('TS','512')); TOTAL_OWN=int(os.environ.get('TO','1024'))
 SCALE = 1.0 / math.sqrt(HEAD_DIM)
+SHARED_PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96)
+OWN_PARTS = (1, 2, 4, 8, 16, 32, 64)
 FEW, MANY = 32, 128    # (row, head) pairs of a workgroup, in the kernel's two roles
 
 
@@ -44,6 +43,96 @@ def _int(x, what: str) -> int:
         return operator.index(x)
     except TypeError:
         raise ValueError("prefix_plan: %s must be whole numbers, got %r" % (what, x)) from None
+
+
+class _Shape:
+    """A batch as tiles of rows, and the ways to cut its pages into parts.
+
+    Shared: a group's rows are cut into tiles that read the shared pages, and every sequence's rows into tiles that read its
+    own.  Alone: every sequence's rows read all of its pages.  A tile is a workgroup per kv head and part: up to 32 pairs of
+    rows and heads, whose wavefronts take 32 keys each, or up to 128, 32 for each wavefront.  More parts are more workgroups
+    and more results to write and to bring together; where every row has one part the second launch falls away."""
+
+    def __init__(self, groups, seqs, n_heads, n_kv, max_ctx):
+        self.n_heads, self.n_kv, self.G, self.R = n_heads, n_kv, n_heads // n_kv, len(seqs)
+        self.pages = -(-max_ctx // PAGE)
+        self.groups, r0 = [], 0          # (pages, tiles of the group, tiles of its sequences): (first row, rows, table)
+        for n, p in groups:
+            r1, runs, a = r0 + n, [], r0
+            while a < r1:
+                b = a + 1
+                while b < r1 and seqs[b] == seqs[a]:
+                    b += 1
+                runs += self._cut(a, b, seqs[a])
+                a = b
+            if len({t for _a, _n, t in runs}) == 1:
+                p = 0                    # one sequence shares with nobody
+            self.groups.append((p, self._cut(r0, r1, seqs[r0]), runs))
+            r0 = r1
+        self.sums = [(p, len(tiles), tiles[0][1] * self.G > FEW, len(runs), any(n * self.G > FEW for _a, n, _t in runs),
+                      sum(n for _a, n, _t in runs)) for p, tiles, runs in self.groups]
+
+    def _cut(self, a, b, table):
+        tile = (FEW if (b - a) * self.G <= FEW else MANY) // self.G
+        return [(i, min(tile, b - i), table) for i in range(a, b, tile)]
+
+    def works(self, share: bool, shared_parts: int, own_parts: int):
+        """(the works, parts of every row)."""
+        works, count = [], [0] * self.R
+        for p, tiles, _runs in self.groups:
+            if share and p:
+                C = min(shared_parts, -(-p // 2))
+                works += [(a, n, t, 0, p, c, C, 0) for c in range(C) for a, n, t in tiles]
+                for a, n, _t in tiles:
+                    count[a:a + n] = [C] * n
+        for p, _tiles, runs in self.groups:
+            p = p if share else 0
+            C = min(own_parts, -(-(self.pages - p) // 2))
+            works += [(a, n, t, p, self.pages, c, C, count[a]) for a, n, t in runs for c in range(C)]
+            for a, n, _t in runs:
+                count[a:a + n] = [count[a] + C] * n
+        return works, count
+
+    def micros(self, share: bool, shared_parts: int, own_parts: int) -> float:
+        """About how long a call takes: a launch and its first loads 4.5 us; a page of a tile of 128 pairs 1.35 us where CUs have
+        one, 2.1 for two together; 32 keys of a wavefront 0.75; bytes at 5 TB/s from memory, 15 from L2; a second launch 2.5,
+        the parts' results 0.5 us per MB, written and read, and 150 ns per 1000 of them brought together.  Over 56 batches of 2
+        to 768 rows behind 128 to 32768 tokens, the cut that it puts first takes 2.4 % longer than the fastest one on average
+        (512 and 1024 workgroups whatever the batch: 29 %)."""
+        many = few = many_pages = few_units = parts = read = loaded = 0
+        for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
+            own = (self.pages - p + 1) // 2       # (contexts end somewhere up to the plan's longest)
+            read += p + runs * own
+            if share and p:
+                todo = ((tiles, tiles_many, p, min(shared_parts, -(-p // 2))),
+                        (runs, runs_many, own, min(own_parts, -(-(self.pages - p) // 2))))
+            else:
+                todo = ((runs, runs_many, p + own, min(own_parts, -(-self.pages // 2))),)
+            for n, is_many, pages, C in todo:
+                if not C:
+                    continue
+                parts += rows * C
+                loaded += n * pages
+                if is_many:
+                    many += n * C * self.n_kv
+                    many_pages = max(many_pages, -(-pages // C))
+                else:
+                    few += n * C * self.n_kv
+                    few_units = max(few_units, -(-pages // (2 * C)))
+        page = self.n_kv * 32768e-6                # MB
+        t_many = many_pages * (1.35 if many <= 256 else 2.1 * max(1.0, many / 512))
+        t_few = few_units * 0.75 * max(1.0, few / 512)
+        t = max(t_many, t_few) if many + few <= 512 else t_many + t_few
+        t = 4.5 + math.hypot(t, read * page / 5, loaded * page / 15)
+        if parts > self.R:
+            t += 2.5 + 0.5e-6 * parts * self.n_heads * 512 + 1.5e-4 * self.R * self.n_heads
+        return t
+
+    def choose(self):
+        ways = [(False, 1, own) for own in OWN_PARTS]
+        if any(p for p, _t, _r in self.groups):
+            ways += [(True, shared, own) for shared in SHARED_PARTS for own in OWN_PARTS]
+        return min(ways, key=lambda way: self.micros(*way))
 
 
 def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None) -> PrefixPlan:
@@ -70,42 +159,8 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     if len(seqs) != R or min(seqs) < 0:
         raise ValueError("prefix_plan: seqs must give a block table (0 ..) to each of the %d rows" % R)
 
-    G = n_heads // n_kv
-    few, many = FEW // G, MANY // G      # rows of a work
-    def cut(a, b):
-        """Rows a .. b - 1 as tiles."""
-        tile = few if (b - a) * G <= FEW else many
-        return [(i, min(tile, b - i)) for i in range(a, b, tile)]
-    if ALONE if ALONE is not None else False:
-        groups = [(r, 0) for r, _ in groups]
-    shared, owned, r0 = [], [], 0        # (first row, rows, table, first page, last page + 1)
-    for n, p in groups:
-        r1 = r0 + n
-        if seqs[r0] == seqs[r1 - 1] and len(set(seqs[r0:r1])) == 1:
-            p = 0                        # one sequence shares with nobody
-        if p:
-            shared.append([(a, k, seqs[r0], 0, p) for a, k in cut(r0, r1)])
-        a = r0
-        while a < r1 and p < pages_max:
-            b = a + 1
-            while b < r1 and seqs[b] == seqs[a]:
-                b += 1
-            owned += [(i, k, seqs[a], p, pages_max) for i, k in cut(a, b)]
-            a = b
-        r0 = r1
-    parts_of = lambda blocks, pages, total: max(1, min(-(-pages // 2), total // max(1, blocks * n_kv)))
-    works, count = [], [0] * R
-    blocks = sum(len(s) for s in shared)
-    for tiles in shared:
-        C = parts_of(blocks, tiles[0][4], TOTAL_SHARED)
-        for c in range(C):
-            works += [(a, n, t, p0, p1, c, C, 0) for a, n, t, p0, p1 in tiles]
-        for a, n, *_ in tiles:
-            count[a:a + n] = [C] * n
-    for a, n, t, p0, p1 in owned:
-        C = 1 if ALONE else parts_of(len(owned), p1 - p0, TOTAL_OWN)
-        works += [(a, n, t, p0, p1, c, C, count[a]) for c in range(C)]
-        count[a:a + n] = [count[a] + C] * n
+    shape = _Shape(groups, seqs, n_heads, n_kv, max_ctx)
+    works, count = shape.works(*shape.choose())
     base = [0]
     for n in count:
         base.append(base[-1] + n)
@@ -113,7 +168,9 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     flat = [x for w in works for x in w] + seqs + base
     flat = torch.tensor(flat, dtype=torch.int32).to(dev)
     n = 8 * len(works)
-    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, count[0] if min(count) == max(count) else 0, base[-1], flat[:n].view(-1, 8), flat[n + R:], flat[n:n + R])
+    even = count[0] if min(count) == max(count) else 0
+    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, even, base[-1], flat[:n].view(-1, 8), flat[n + R:],
+                      flat[n:n + R])
 
 
 def prefix_workspace(plan: PrefixPlan) -> tuple:

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from p2p_llm_chat_go_amd import ops
+from p2p_llm_chat_go_amd.ops import prefix
 from tests import prefix_oracle as oracle
 
 PAGE, D = 64, 128
@@ -27,9 +28,13 @@ def test_plans_that_are_refused(why, call):
         call()
 
 
-def test_whatever_the_cut_every_key_of_a_row_is_in_one_part():
+@pytest.mark.parametrize("way", [None, (True, 1, 1), (True, 3, 1), (True, 48, 8), (False, 1, 1), (False, 1, 16)])
+def test_whatever_the_cut_every_key_of_a_row_is_in_one_part(way, monkeypatch):
+    """way: the cut (None: the one that the plan chooses)."""
+    if way is not None:
+        monkeypatch.setattr(prefix._Shape, "choose", lambda self: way)
     rng = random.Random(0)
-    for _ in range(60):
+    for _ in range(30):
         kv = rng.choice([1, 2, 8])
         heads = kv * rng.choice([1, 2, 3, 4, 8, 32])
         groups, seqs, s = [], [], 0
@@ -43,6 +48,8 @@ def test_whatever_the_cut_every_key_of_a_row_is_in_one_part():
         most = rng.randint(30 * PAGE, 40 * PAGE)
         plan = _plan(groups, heads, kv, most, seqs=seqs)
         R = len(seqs)
+        counts = (plan.base[1:] - plan.base[:-1]).tolist()
+        assert min(counts) >= 1 and plan.even == (counts[0] if len(set(counts)) == 1 else 0)
         assert plan.rows == R and plan.base[-1] == plan.parts and plan.row_tables.tolist() == seqs
         first, parts = [0] * R, [[] for _ in range(R)]
         at = 0

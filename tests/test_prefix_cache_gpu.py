@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from p2p_llm_chat_go_amd import ops
+from p2p_llm_chat_go_amd.ops import prefix
 from p2p_llm_chat_go_amd.models.config import LLAMA31_8B, rope_table
 from tests import prefix_oracle as oracle
 
@@ -59,13 +60,24 @@ def _run(q, k, v, table, ctx, plan, **kw):
     return ops.prefix_attention(q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), ctx.to(DEV), plan, **kw)
 
 
+# cuts of a batch (shared pages or not, parts of them, parts of a sequence's own pages); None: the one that the plan chooses
+WAYS = [None, (True, 1, 1), (True, 5, 2), (False, 1, 1), (False, 1, 3)]
+
+
+@pytest.fixture(params=WAYS, ids=str)
+def way(request, monkeypatch):
+    if request.param is not None:
+        monkeypatch.setattr(prefix._Shape, "choose", lambda self: request.param)
+    return request.param
+
+
 HEADS = [(8, 1), (8, 2), (4, 4), (6, 2), (16, 1), (32, 1), (5, 1)]
 
 
 @pytest.mark.parametrize("Hq,Hkv", HEADS)
 @pytest.mark.parametrize("groups,own", [([(2, 1)], 1), ([(1, 2)], 70), ([(3, 0)], 65), ([(7, 3), (1, 0), (20, 5), (2, 1)], 130),
                                         ([(70, 9)], 33), ([(5, 40)], 300)])
-def test_prefix_attention_of_decode_rows(Hq, Hkv, groups, own):
+def test_prefix_attention_of_decode_rows(way, Hq, Hkv, groups, own):
     q, k, v, table, seqs, ctx, rows, most = _batch(groups, Hq, Hkv, own, Hq + own)
     plan = ops.prefix_plan(rows, Hq, Hkv, most, DEV)
     want, bound = oracle.attention(q, k, v, table, seqs, ctx, Hq, Hkv, 1 / math.sqrt(D), most)
@@ -73,8 +85,9 @@ def test_prefix_attention_of_decode_rows(Hq, Hkv, groups, own):
 
 
 @pytest.mark.parametrize("groups,own", [([(2, 560)], 9), ([(40, 150)], 3), ([(1, 0), (2, 700)], 2)])
-def test_prefix_attention_in_many_parts(groups, own):
+def test_prefix_attention_in_many_parts(groups, own, monkeypatch):
     """One kv head: up to some 300 parts of a row."""
+    monkeypatch.setattr(prefix._Shape, "choose", lambda self: (True, 400, 100))
     q, k, v, table, seqs, ctx, rows, most = _batch(groups, 8, 1, own, own)
     plan = ops.prefix_plan(rows, 8, 1, most, DEV)
     want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 1, 1 / math.sqrt(D), most)
@@ -84,7 +97,7 @@ def test_prefix_attention_in_many_parts(groups, own):
 @pytest.mark.parametrize("Hq,Hkv", [(8, 2), (4, 4), (8, 1), (3, 1)])
 @pytest.mark.parametrize("groups,own,tokens", [([(3, 2)], 44, 44), ([(2, 4), (3, 1)], 100, 17), ([(1, 5)], 200, 130),
                                                ([(9, 1)], 64, 2)])
-def test_prefix_attention_of_prompt_rows(Hq, Hkv, groups, own, tokens):
+def test_prefix_attention_of_prompt_rows(way, Hq, Hkv, groups, own, tokens):
     q, k, v, table, seqs, ctx, rows, most = _batch(groups, Hq, Hkv, own, tokens, tokens)
     plan = ops.prefix_plan(rows, Hq, Hkv, most, DEV, seqs=seqs)
     want, bound = oracle.attention(q, k, v, table, seqs, ctx, Hq, Hkv, 0.2, most)
@@ -92,7 +105,7 @@ def test_prefix_attention_of_prompt_rows(Hq, Hkv, groups, own, tokens):
 
 
 @pytest.mark.parametrize("Hq,Hkv", [(8, 2), (2, 2)])
-def test_rows_that_see_nothing_part_of_the_prefix_or_more_than_the_plan(Hq, Hkv):
+def test_rows_that_see_nothing_part_of_the_prefix_or_more_than_the_plan(way, Hq, Hkv):
     """Contexts of 0 and less give zeros; a context may end inside the shared pages, at any key of a page; what lies past the
     plan's longest context is not read."""
     q, k, v, table, seqs, ctx, rows, most = _batch([(24, 3), (3, 0)], Hq, Hkv, 40, 5)
@@ -109,7 +122,7 @@ def test_rows_that_see_nothing_part_of_the_prefix_or_more_than_the_plan(Hq, Hkv)
 
 
 @pytest.mark.parametrize("tokens", [1, 20])
-def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(tokens):
+def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(way, tokens):
     q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 3, tokens)
     if tokens == 1:
         ctx[:12] = torch.arange(100, 124, 2, dtype=torch.int32)
@@ -129,7 +142,7 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(tokens):
     assert float(far.max()) <= 0
 
 
-def test_rows_and_tables_of_any_stride_and_rows_behind_the_plan():
+def test_rows_and_tables_of_any_stride_and_rows_behind_the_plan(way):
     q, k, v, table, seqs, ctx, rows, most = _batch([(9, 2)], 8, 2, 50, 9)
     wide = torch.randn(12, 8 * D + 3).bfloat16()
     wide[:9, 1:1 + 8 * D] = q
@@ -155,7 +168,7 @@ def test_pages_outside_of_the_cache_are_read_inside_it():
     _check(_run(q, k, v, table, ctx, plan), ref, bound)
 
 
-def test_one_plan_serves_a_captured_step_while_contexts_grow():
+def test_one_plan_serves_a_captured_step_while_contexts_grow(way):
     """Two graphs with a workspace each, replayed in turn with eager work between; every replay is as the eager call."""
     q, k, v, table, seqs, ctx, rows, most = _batch([(11, 3), (4, 1)], 8, 2, 150, 21)
     k, v = k.nan_to_num(0.5), v.nan_to_num(0.5)
