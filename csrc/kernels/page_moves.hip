@@ -105,23 +105,24 @@ __global__ __launch_bounds__(256) void compact_apart_kernel(Cache k, Cache v, Se
   if (p0 >= len && p0 > 0) return;
   const uint8_t* keep = s.keep + seq * s.keep_stride;
   __shared__ int count[4];
-  __shared__ uint8_t set[TOK];
   int before = 0;
   for (int j = tid * 8; j < p0; j += 256 * 8) before += set_of_8(keep + j);   // p0 is a multiple of 8
   const bool kept = place < len && keep[place] != 0;
-  if (part == 0) set[t] = kept;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
-  if ((tid & 63) == 0) count[tid >> 6] = before;
+  __shared__ int here[4];                                    // kept places of a wavefront
+  const unsigned long long set = __ballot(kept && part == 0);   // one lane per place
+  const int w = tid >> 6, lane = tid & 63;
+  if (lane == 0) {
+    count[w] = before;
+    here[w] = __popcll(set);
+  }
   __syncthreads();
   int to = count[0] + count[1] + count[2] + count[3];
-  if (last && blockIdx.z == 0 && tid == 0) {
-    int n = to;
-    for (int j = 0; j < TOK; ++j) n += set[j];
-    s.new_lens[seq] = n;
-  }
+  if (last && blockIdx.z == 0 && tid == 0) s.new_lens[seq] = to + here[0] + here[1] + here[2] + here[3];
   if (!kept) return;
-  for (int j = 0; j < t; ++j) to += set[j];
+  for (int x = 0; x < w; ++x) to += here[x];
+  to += __popcll(set & ((1ull << (lane - part)) - 1));
   const int from_page = s.tables[(long)seq * s.table_stride + place / PAGE], to_page = s.to[(long)seq * s.to_stride + to / PAGE];
   if ((unsigned)from_page >= (unsigned)s.num_pages || (unsigned)to_page >= (unsigned)s.num_pages) return;
   Turn turn;
@@ -141,53 +142,98 @@ __global__ __launch_bounds__(256) void compact_apart_kernel(Cache k, Cache v, Se
   }
 }
 
-// In place: one workgroup moves all of a sequence's tokens of one head, 1024 / TPT places after the other.  A place n takes the
-// token of a place p >= n, so once the workgroup has read its places no later read meets what it writes.
-template <int TPT, bool TURN>
+// In place: one workgroup moves all of a sequence's tokens of HEADS heads, a round of 1024 / TPT places after the other.  A place
+// n takes the token of a place p >= n: once the workgroup has read a round's places no later read meets what it writes, and the
+// next round's reads go out before this one's writes.
+template <int TPT, bool TURN, int HEADS>
 __global__ __launch_bounds__(1024) void compact_inside_kernel(Cache k, Cache v, Sequences s, int heads,
                                                               const float* __restrict__ cos_sin) {
   constexpr int TOK = 1024 / TPT, HALF = TPT * 16;
-  const int seq = blockIdx.y, h = blockIdx.x % heads, layer = blockIdx.x / heads;
-  const int tid = threadIdx.x, t = tid / TPT, part = tid % TPT;
+  const int seq = blockIdx.y, h0 = blockIdx.x % (heads / HEADS) * HEADS, layer = blockIdx.x / (heads / HEADS);
+  const int tid = threadIdx.x, t = tid / TPT, part = tid % TPT, w = tid >> 6, lane = tid & 63;
   const int len = length_of(s, seq);
   const uint8_t* keep = s.keep + seq * s.keep_stride;
   const int* table = s.tables + (long)seq * s.table_stride;
-  char* kp = k.p + layer * k.layer + h * k.head + part * 16;
-  char* vp = v.p + layer * v.layer + h * v.head + part * 16;
-  __shared__ uint8_t set[2][TOK];
-  int base = 0, side = 0;
-  for (int p0 = 0; p0 < len; p0 += TOK, side ^= 1) {
-    const int place = p0 + t;
-    bool kept = place < len && keep[place] != 0;
-    if (part == 0) set[side][t] = kept;
-    __syncthreads();
-    int to = base;
-    for (int j = 0; j < TOK; ++j) {
-      const int one = set[side][j];
-      base += one;
-      if (j < t) to += one;
+  char* kp = k.p + layer * k.layer + h0 * k.head + part * 16;
+  char* vp = v.p + layer * v.layer + h0 * v.head + part * 16;
+  __shared__ int here[2][16];   // kept places of a wavefront, of this round and the one before
+  __shared__ int start;
+  // the pages: in LDS (a round waits for its places' new pages), those of longer sequences where they are
+  constexpr int PAGES = 4096;
+  __shared__ int pages[PAGES];
+  for (int i = tid; i < min((len + PAGE - 1) / PAGE, PAGES); i += 1024) pages[i] = table[i];
+  const auto page_of = [&](int place) {
+    const int i = place / PAGE;
+    return i < PAGES ? pages[i] : table[i];
+  };
+  // the places before the first that is not kept stay: rounds begin there
+  if (tid == 0) start = len;
+  __syncthreads();
+  int mine = len;
+  for (int p = tid * 8; p < len; p += 1024 * 8) {
+    if (p + 8 <= len && set_of_8(keep + p) == 8) continue;
+    mine = p;
+    break;
+  }
+  if (mine < len) atomicMin(&start, mine);
+  __syncthreads();
+  int base = start < len ? start / TOK * TOK : len, side = 0;   // kept places before the round, all of them until here
+
+  bool kept = false, next_kept = false;   // this thread's place of a round, of the next
+  const auto look = [&](int p0) { return p0 + t < len && keep[p0 + t] != 0; };
+  Row a[HEADS], b[HEADS];
+  const auto load = [&](int p0, bool is) {
+    const int pg = is ? page_of(p0 + t) : -1;
+    if ((unsigned)pg >= (unsigned)s.num_pages) return;
+    const long in = (long)((p0 + t) % PAGE) * 2 * HALF;
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      a[h] = load_row(kp + h * k.head + pg * k.page + in, HALF);
+      b[h] = load_row(vp + h * v.head + pg * v.page + in, HALF);
     }
-    const int from_page = kept ? table[place / PAGE] : 0, to_page = kept ? table[to / PAGE] : 0;
-    kept = kept && to != place && (unsigned)from_page < (unsigned)s.num_pages && (unsigned)to_page < (unsigned)s.num_pages;
-    Row a, b;
-    if (kept) {
-      const long in = (long)(place % PAGE) * 2 * HALF;
-      a = load_row(kp + from_page * k.page + in, HALF);
-      b = load_row(vp + from_page * v.page + in, HALF);
-      if constexpr (TURN) {
-        Turn turn;
-        turn.set(cos_sin, place, to, part * 8);
-        turn.apply(a);
-      }
+  };
+  const int p_first = base;
+  kept = look(p_first);
+  load(p_first, kept);
+  for (int p0 = p_first; p0 < len; p0 += TOK, side ^= 1) {
+    const int place = p0 + t;
+    next_kept = look(p0 + TOK);
+    const unsigned long long set = __ballot(kept && part == 0);   // one lane per place
+    if (lane == 0) here[side][w] = __popcll(set);
+    __syncthreads();
+    int to = base + __popcll(set & ((1ull << (lane - part)) - 1));
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int n = here[side][x];
+      base += n;
+      if (x < w) to += n;
+    }
+    const int to_page = kept ? page_of(to) : -1;
+    const bool moves = kept && to != place && (unsigned)to_page < (unsigned)s.num_pages
+                       && (unsigned)page_of(place) < (unsigned)s.num_pages;
+    Turn turn;
+    if constexpr (TURN)
+      if (moves) turn.set(cos_sin, place, to, part * 8);
+    Row x[HEADS], y[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      x[h] = a[h];
+      y[h] = b[h];
     }
     // every wavefront's loads have come back before any writes
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (kept) {
+    load(p0 + TOK, next_kept);
+    if (moves) {
       const long in = (long)(to % PAGE) * 2 * HALF;
-      store_row(kp + to_page * k.page + in, HALF, a);
-      store_row(vp + to_page * v.page + in, HALF, b);
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) {
+        if constexpr (TURN) turn.apply(x[h]);
+        store_row(kp + h * k.head + to_page * k.page + in, HALF, x[h]);
+        store_row(vp + h * v.head + to_page * v.page + in, HALF, y[h]);
+      }
     }
+    kept = next_kept;
   }
   if (blockIdx.x == 0 && tid == 0) s.new_lens[seq] = base;
 }
@@ -195,12 +241,18 @@ __global__ __launch_bounds__(1024) void compact_inside_kernel(Cache k, Cache v, 
 template <int TPT, bool TURN>
 int compact(Cache k, Cache v, const Sequences& s, int n, int heads, int layers, const float* cos_sin, hipStream_t st) {
   if (!s.to) {
-    hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN>), dim3(heads * layers, n), dim3(1024), 0, st, k, v, s, heads, cos_sin);
+    const int groups = heads * layers * n;
+    constexpr int MANY = TURN ? 2 : 1;
+    if (MANY > 1 && heads % MANY == 0 && groups / MANY >= 192)
+      hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN, MANY>), dim3(heads / MANY * layers, n), dim3(1024), 0, st, k, v, s, heads,
+                         cos_sin);
+    else
+      hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN, 1>), dim3(heads * layers, n), dim3(1024), 0, st, k, v, s, heads, cos_sin);
     return (int)hipGetLastError();
   }
   constexpr int TOK = 256 / TPT;
   const int chunks = max(1, (min(s.places, s.width * PAGE) + TOK - 1) / TOK);
-  const int shares = max(1, min(heads * layers, 2048 / max(1, chunks * n)));
+  const int shares = max(1, min(heads * layers / 8, 8192 / max(1, chunks * n)));
   hipLaunchKernelGGL((compact_apart_kernel<TPT, TURN>), dim3(chunks, n, shares), dim3(256), 0, st, k, v, s, heads, layers, cos_sin);
   return (int)hipGetLastError();
 }
