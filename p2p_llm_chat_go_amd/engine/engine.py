@@ -47,6 +47,16 @@ def bucket(x, buckets):
     raise ValueError("%d exceeds the largest bucket %d" % (x, buckets[-1]))
 
 
+def common_prefix(prompts: list) -> int:
+    """Tokens that all prompts begin with, short of the shortest prompt's last one."""
+    n = min(len(p) for p in prompts) - 1
+    first = prompts[0]
+    for p in prompts[1:]:
+        if p[:n] != first[:n]:
+            n = next(i for i in range(n) if p[i] != first[i])
+    return max(n, 0)
+
+
 @dataclasses.dataclass
 class GenResult:
     tokens: list
@@ -108,6 +118,7 @@ class Engine:
         self.use_graph = use_graph
         self._prefill_ws = {}
         self._graphs = {}
+        self._shared_graphs = {}     # decode graphs of batches that share pages, the last one of every bucket
         # graph-captured prefill chunks (engine.graph.PrefillGraph): dense TP=1 engines on
         # the GPU; P2P_PREFILL_GRAPH=0 keeps every prefill eager
         # TP groups: chunks whose every collective runs on the one-shot IPC kernels (the
@@ -150,6 +161,18 @@ class Engine:
             g = DecodeGraph(st, self.use_graph, greedy=greedy).capture()
             self._graphs[key] = g
         return g
+
+    def shared_decode_graph(self, B: int, ctx: int, pages: int) -> DecodeGraph:
+        """The greedy decode graph of B sequences that begin with the same ``pages`` pages (ops.prefix_attention)."""
+        key = (bucket(B, BATCH_BUCKETS), bucket(ctx, CTX_BUCKETS))
+        have = self._shared_graphs.get(key)
+        if have is None or have[0] != (B, pages):
+            self._shared_graphs.pop(key, None)
+            st = DecodeState(self.model, key[0], key[1] // PAGE, key[1], key[1])
+            plan = ops.prefix_plan([(B, pages)] + [(1, 0)] * (key[0] - B), self.model.nq, self.model.nkv, key[1], self.device)
+            st.prefix = {"prefix": (plan, ops.prefix_workspace(plan))}
+            have = self._shared_graphs[key] = ((B, pages), DecodeGraph(st, self.use_graph).capture())
+        return have[1]
 
     def prefill_graph_key(self, rows: int, n_seq: int, max_ctx: int, greedy: bool = True):
         return (bucket(rows, PREFILL_ROW_BUCKETS), min(bucket(n_seq, BATCH_BUCKETS), self.max_batch),
@@ -225,7 +248,7 @@ class Engine:
     # -------------------------------------------------------------- prefill
     def prefill(self, prompts: list, block_tables: list, return_logits: bool = False,
                 sampling: list | None = None, starts: list | None = None,
-                pad_rows: int | None = None, graph: bool = True):
+                pad_rows: int | None = None, graph: bool = True, shared_pages: int = 0):
         """Run all prompts (flat rows, chunked at max_prefill_tokens); ``graph=False``
         keeps it off the captured-chunk path (the native loop owns that policy).
 
@@ -239,7 +262,11 @@ class Engine:
         pad_rows: run exactly this many rows (>= the real ones), the rest dummy rows of an
         extra sequence on the KV null page -- EP all-to-all ranks serving different
         sequences (DP attention) must run the same chunks with equal row counts.
+        shared_pages: all block tables begin with the same so many pages, which hold tokens before
+        every sequence's start: their keys are read once for all rows (ops.prefix_attention).
         """
+        if shared_pages and (pad_rows is not None or any(s0 < shared_pages * PAGE for s0 in starts or [0])):
+            raise ValueError("prefill: shared pages hold tokens before every start, without dummy rows")
         sampled = sampling is not None and not all(p.greedy for p in sampling)
         dev = self.device
         B = len(prompts)
@@ -253,7 +280,7 @@ class Engine:
             assert n_dummy >= 0, (pad_rows, len(rows))
             rows += [(B, i, 0) for i in range(n_dummy)]  # sequence B: the null page
         max_ctx = max([len(p) for p in prompts] + [n_dummy, 1])
-        if (graph and self._graph_prefill_ok(len(rows), B, max_ctx, n_dummy, return_logits) and
+        if (graph and not shared_pages and self._graph_prefill_ok(len(rows), B, max_ctx, n_dummy, return_logits) and
                 self.prefill_graph_wanted(self.prefill_graph_key(len(rows), B, max_ctx,
                                                                  not sampled))):
             return self._prefill_graphed(prompts, block_tables, rows, max_ctx, sampling, sampled)
@@ -284,8 +311,11 @@ class Engine:
                     outs.append(j)
                     out_seq.append(b)
             greedy = all_logits is None and not sampled
-            tiles_h = qtile = None
-            if self.flash_prefill_min and R >= self.flash_prefill_min:
+            tiles_h = qtile = prefix = None
+            if shared_pages:
+                plan = ops.prefix_plan([(R, shared_pages)], self.model.nq, self.model.nkv, max_ctx, dev, seqs=seq)
+                prefix = plan, ops.prefix_workspace(plan)
+            elif self.flash_prefill_min and R >= self.flash_prefill_min:
                 qtile = ops.flash_tile(self.model.nq, self.model.nkv, R, self.cfg.is_moe,
                                        chunk[-1][0] - chunk[0][0] + 1, int(pos.max()) + 1)
                 tiles_h = ops.prefill_tiles(seq.tolist(), pos.tolist(), qtile)
@@ -309,7 +339,8 @@ class Engine:
             tiles = None if tiles_h is None else dev_all[o:o + tiles_h.numel()].view(tiles_h.shape)
             res = self.model.forward(ws, ids_d, pos_d, slots_d, bt_d, seq_d, ctx_d, R,
                                      max_ctx, out_rows=out_rows, n_out=len(outs), greedy=greedy,
-                                     tiles=tiles, tiles_host=tiles_h, qtile=qtile)
+                                     tiles=tiles, tiles_host=tiles_h, qtile=qtile,
+                                     **({"prefix": prefix} if prefix else {}))
             if not outs:
                 continue
             if greedy:
@@ -376,16 +407,31 @@ class Engine:
 
     # ------------------------------------------------------------- generate
     def generate(self, prompts: list, max_new_tokens: int = 64, stop_on_eos: bool = True,
-                 check_every: int = 8) -> list:
-        """Greedy suggest-reply for a static batch of prompts (token id lists)."""
+                 check_every: int = 8, share_prefix: bool = False) -> list:
+        """Greedy suggest-reply for a static batch of prompts (token id lists).
+
+        share_prefix: the tokens that all prompts begin with are run once, and the sequences share
+        their full pages of the cache (``KVCache.fork``); attention reads those once for the batch
+        (``ops.prefix_attention``).  The numbers are the same up to the order of sums.  Prompts
+        that have less than a page in common run as without it."""
         t0 = time.perf_counter_ns()
         B = len(prompts)
         assert 0 < B <= self.max_batch
         need = [len(p) + max_new_tokens for p in prompts]
-        pages = [self.kv.allocator.alloc(pages_for(n)) for n in need]
+        shared = common_prefix(prompts) if share_prefix and B > 1 else 0
+        if shared < PAGE:
+            shared = 0
+        pages = []
         try:
-            with span("prefill", batch=B, tokens=sum(len(p) for p in prompts)):
-                first = self.prefill(prompts, pages)
+            for n in need[:1] if shared else need:
+                pages.append(self.kv.allocator.alloc(pages_for(n)))
+            with span("prefill", batch=B, tokens=sum(len(p) for p in prompts) - shared * (B - 1)):
+                if shared:
+                    self.prefill([prompts[0][:shared]], pages)
+                    pages += self.kv.fork(pages[0], shared, [pages_for(n) for n in need[1:]])
+                    first = self.prefill(prompts, pages, starts=[shared] * B, shared_pages=shared // PAGE)
+                else:
+                    first = self.prefill(prompts, pages)
                 first_h = first.cpu()  # sync: first token is on the host -> TTFT
             self.check_comm()
             t1 = time.perf_counter_ns()
@@ -394,7 +440,7 @@ class Engine:
             n_dec = max_new_tokens - 1
             steps_run = 0
             if n_dec > 0 and not all(done):
-                g = self.decode_graph(B, max(need))
+                g = self.shared_decode_graph(B, max(need), shared // PAGE) if shared else self.decode_graph(B, max(need))
                 st = g.state
                 st.load([o[0] for o in out], [len(p) for p in prompts], pages)
                 while steps_run < n_dec:

@@ -48,6 +48,7 @@ class DecodeState:
         self.ws = model.new_workspace(B, max_ctx)
         self.samp = SamplerSlots(B, dev, self.image, at)  # sampled graphs read these (ops.sample)
         self._report = None
+        self.prefix = {}     # forward's ``prefix``, where the rows share pages (Engine.generate)
         if model.tp > 1:  # vocab-parallel sampling: per-shard top-128 candidates, gathered
             W = model.tp
             self.cand_v = torch.empty(B, 128, device=dev, dtype=torch.float32)
@@ -103,7 +104,7 @@ class DecodeState:
     def body_logits(self):
         """Forward only (sampling mode): logits of every row in ws.logits."""
         self.model.forward(self.ws, self.ids, self.pos, self.slots, self.bt, None,
-                           self.ctx, self.B, self.max_ctx)
+                           self.ctx, self.B, self.max_ctx, **self.prefix)
 
     def advance(self):
         ops.advance(self.ids, self.pos, self.ctx, self.slots, self.bt, self.hist, self.step)
@@ -135,7 +136,7 @@ class DecodeState:
     def body(self):
         m = self.model
         keys = m.forward(self.ws, self.ids, self.pos, self.slots, self.bt, None, self.ctx,
-                         self.B, self.max_ctx, greedy=True)
+                         self.B, self.max_ctx, greedy=True, **self.prefix)
         if m.tp > 1:
             m.comm.allreduce_max_u64_(keys[:self.B])
         # keys -> ids (+ reset) folded into the state advance: no extra launch

@@ -7,15 +7,21 @@ wave streams).  Page 0 is reserved as the *null page*: padding rows of a
 graph batch bucket write and read there, so bucketed graphs never touch a
 live sequence.
 
+Sequences may share pages: :meth:`KVCache.fork` gives a new sequence the full pages of the tokens it begins with and a
+copy of the page that both go on writing to; a page returns to the free list when its last owner frees it.
+:meth:`KVCache.compact` moves the tokens that a sequence keeps together and frees the pages behind them.
+
 On a 288 GB MI355X, llama3.1-8B leaves ~270 GB for KV = ~2.1 M tokens at
 128 KiB/token; the default fraction below keeps headroom for workspaces.
 """
 from __future__ import annotations
 
+import collections
+
 import torch
 
 from ..models.config import ModelConfig
-from ..ops import HEAD_DIM, PAGE
+from ..ops import HEAD_DIM, PAGE, compact_pages, copy_pages
 
 
 class PageAllocator:
@@ -28,10 +34,23 @@ class PageAllocator:
             raise ValueError("need at least 2 pages (page 0 is the null page)")
         self.num_pages = num_pages
         self._free = list(range(num_pages - 1, 0, -1))
+        self._more = {}      # page -> owners beyond the first
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def shared(self, page: int) -> bool:
+        """Whether more than one sequence owns the page."""
+        return page in self._more
+
+    def share(self, pages):
+        """One more owner for each of the pages (which are in use); each owner frees them once."""
+        for p in pages:
+            if p <= 0 or p >= self.num_pages:
+                raise ValueError("bad page %d" % p)
+        for p in pages:
+            self._more[p] = self._more.get(p, 0) + 1
 
     def alloc(self, n: int) -> list:
         if n > len(self._free):
@@ -43,7 +62,14 @@ class PageAllocator:
         for p in pages:
             if p <= 0 or p >= self.num_pages:
                 raise ValueError("bad page %d" % p)
-        self._free.extend(pages)
+        for p in pages:
+            more = self._more.get(p)
+            if more is None:
+                self._free.append(p)
+            elif more == 1:
+                del self._more[p]
+            else:
+                self._more[p] = more - 1
 
 
 def pages_for(tokens: int) -> int:
@@ -82,3 +108,72 @@ class KVCache:
 
     def layer(self, i: int):
         return self.k[i], self.v[i]
+
+    def fork(self, pages: list, tokens: int, sizes: list) -> list:
+        """Page lists of ``len(sizes)`` new sequences that begin with the first ``tokens`` tokens of ``pages``, of sizes[i]
+        pages each.  Full pages of those tokens are shared; of a last page that is not full every new sequence gets a copy
+        (``ops.copy_pages``, all layers in one launch).  Whoever goes on writing to ``pages`` does so behind ``tokens``."""
+        if not 0 <= tokens <= len(pages) * PAGE:
+            raise ValueError("fork: %d tokens of %d pages" % (tokens, len(pages)))
+        full, need = tokens // PAGE, pages_for(tokens)
+        if any(n < need for n in sizes):
+            raise ValueError("fork: %d tokens take %d pages, asked for %d" % (tokens, need, min(sizes)))
+        fresh = self.allocator.alloc(sum(n - full for n in sizes))
+        out, at = [], 0
+        for n in sizes:
+            self.allocator.share(pages[:full])
+            out.append(list(pages[:full]) + fresh[at:at + n - full])
+            at += n - full
+        if need > full:
+            copy_pages(self.k, self.v, [pages[full]] * len(out), [p[full] for p in out], [tokens % PAGE] * len(out))
+        return out
+
+    def compact(self, pages: list, lens: list, keep, cos_sin=None, room: int = 0) -> tuple:
+        """Sequences (their page lists and lengths) reduced to the tokens that ``keep`` ([sequences, tokens], true or false)
+        keeps: (page lists, lengths) of what is left, with pages for ``room`` more tokens each.
+
+        A sequence whose pages are its own is compacted in place, one that shares pages with others (``fork``) into new
+        ones; pages that nobody owns any more are free.  cos_sin (``LlamaModel.rope``): keys are turned to their new
+        positions, and the sequence goes on at its new length; None: it goes on counting from where it was, and only the
+        cache's places change."""
+        dev = self.k.device
+        keep = torch.as_tensor(keep, dtype=torch.bool)
+        if keep.dim() != 2 or keep.shape[0] != len(pages) or len(lens) != len(pages):
+            raise ValueError("compact: %d sequences, %d lengths, keep %s" % (len(pages), len(lens), list(keep.shape)))
+        for p, n in zip(pages, lens):
+            if not 0 <= n <= min(len(p) * PAGE, keep.shape[1]):
+                raise ValueError("compact: a length of %d with %d pages and %d places in keep" % (n, len(p), keep.shape[1]))
+        given = collections.Counter(p for q in pages for p in q)
+        if any(n > 1 and not self.allocator.shared(p) for p, n in given.items()):
+            raise ValueError("compact: a page is given twice")
+        if not pages:
+            return [], []
+        lens_t = torch.tensor(lens, dtype=torch.int32)
+        host = keep.cpu()
+        left = (host & (torch.arange(host.shape[1]) < lens_t[:, None])).sum(1).tolist()
+        size = [pages_for(n + room) for n in left]
+        apart = [any(self.allocator.shared(p) for p in q) for q in pages]
+        # new pages first: nothing has changed when there are none
+        fresh = self.allocator.alloc(sum(n if a else max(0, n - len(q)) for n, a, q in zip(size, apart, pages)))
+        out, gone = [], []
+        for n, a, q in zip(size, apart, pages):
+            take = n if a else max(0, n - len(q))
+            mine, fresh = fresh[:take], fresh[take:]
+            out.append(mine if a else q[:n] + mine)
+            gone += q if a else q[n:]
+        keep = keep.to(dev)
+        for way in (False, True):
+            at = [i for i, a in enumerate(apart) if a == way and lens[i]]
+            if not at:
+                continue
+            width = max(len(pages[i]) for i in at)
+            table = torch.zeros(2, len(at), width, dtype=torch.int32)
+            for j, i in enumerate(at):
+                table[0, j, :len(pages[i])] = torch.tensor(pages[i], dtype=torch.int32)
+                here = out[i][:width]
+                table[1, j, :len(here)] = torch.tensor(here, dtype=torch.int32)
+            table = table.to(dev)
+            compact_pages(self.k, self.v, table[0], lens_t[at].to(dev), keep[torch.tensor(at, device=dev)],
+                          out_tables=table[1] if way else None, cos_sin=cos_sin)
+        self.allocator.free(gone)
+        return out, left

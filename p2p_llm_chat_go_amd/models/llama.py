@@ -191,7 +191,7 @@ class LlamaModel:
 
     def forward(self, ws: Workspace, ids, pos, slots, block_tables, row_bt, ctx_lens, R: int,
                 max_ctx: int, out_rows=None, n_out: int | None = None, greedy: bool = False,
-                tiles=None, tiles_host=None, qtile=None):
+                tiles=None, tiles_host=None, qtile=None, prefix=None):
         """Run all layers on R query rows.
 
         out_rows: int32 [n_out] indices of rows whose logits are needed (prefill:
@@ -201,22 +201,24 @@ class LlamaModel:
         tiles: int32 [n, 4] prefill query tiles (ops.prefill_tiles) -> causal
         attention runs on the MFMA flash-prefill kernel instead of per row.
         row_bt: block-table row of each query row; None = row r uses row r (decode).
+        prefix: (plan, workspace) of ops.prefix_attention, whose plan names the same block-table
+        rows -> sequences that share their first pages read them together.
         """
         cfg = self.cfg
         h = ws.h[:R]
         ops.gather_rows(self.w.embed, ids[:R], out=h)
         if (self.decode_engine and tiles is None and row_bt is None and out_rows is None
-                and self._decode_engine_ok(R, max_ctx)):
+                and prefix is None and self._decode_engine_ok(R, max_ctx)):
             self._de.run(h, pos[:R], slots[:R], self.rope, block_tables, ctx_lens[:R], ws.err)
             return self._head(ws, h, R, out_rows, n_out, greedy)
         q, attn = ws.q[:R], ws.attn[:R]
-        fused = (self.fuse_attn_oproj and tiles is None and self.tp == 1
+        fused = (self.fuse_attn_oproj and tiles is None and prefix is None and self.tp == 1
                  and self.device.type == "cuda" and isinstance(self.w.layers[0].o, torch.Tensor)
                  and ops.attn_oproj_ok(R, self.nq, self.nkv, max_ctx, cfg.hidden))
-        heads = (not fused and self.fuse_heads and tiles is None and ws.heads_slab is not None
+        heads = (not fused and self.fuse_heads and tiles is None and prefix is None and ws.heads_slab is not None
                  and R <= self.heads_max_rows and isinstance(self.w.layers[0].o, torch.Tensor)
                  and ops.attn_oproj_heads_ok(R, self.nq, self.nkv, max_ctx, cfg.hidden))
-        qa = (self.fuse_qkv_attn and not fused and not heads and tiles is None
+        qa = (self.fuse_qkv_attn and not fused and not heads and tiles is None and prefix is None
               and row_bt is None and ws.qa is not None and isinstance(self.w.layers[0].qkv, torch.Tensor)
               and ops.qkv_attn_ok(R, self.nq, self.nkv, max_ctx))
         qa_o = (qa and self.fuse_qkv_attn_oproj and self.tp == 1
@@ -248,7 +250,9 @@ class LlamaModel:
                 ops.attn_oproj(q, kc, vc, block_tables, rb, ctx_lens[:R], self.nq,
                                self.nkv, max_ctx, lw.o, h, attn, ws.sync, ws.err)
             else:
-                if tiles is not None:
+                if prefix is not None:
+                    ops.prefix_attention(q, kc, vc, block_tables, ctx_lens, prefix[0], out=attn, workspace=prefix[1])
+                elif tiles is not None:
                     ops.flash_prefill(q, kc, vc, block_tables, tiles, self.nq, self.nkv, out=attn,
                                       tiles_host=tiles_host, qtile=qtile)
                 else:

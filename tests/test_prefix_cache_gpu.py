@@ -348,6 +348,20 @@ def test_compaction_skips_entries_that_are_no_pages(apart):
     assert torch.equal(kd.cpu().double(), want_k) and torch.equal(vd.cpu().double(), want_v)
 
 
+def test_compaction_of_a_sequence_of_more_pages_than_a_workgroup_holds():
+    """263000 tokens in place, of which three leave: behind them all move."""
+    n, W = 263000, 4110
+    k, v = (torch.randn(1, W + 1, 1, PAGE, D, device=DEV).bfloat16() for _ in range(2))
+    table = (torch.randperm(W, device=DEV).int() + 1)[None]
+    gone = torch.tensor([261990, 262200, 262999], device=DEV)
+    keep = torch.ones(1, n, dtype=torch.bool, device=DEV)
+    keep[0, gone] = False
+    flat = lambda c: c[0, :, 0][table[0].long()].reshape(-1, D)
+    want = [flat(c)[:n][keep[0]] for c in (k, v)]
+    assert ops.compact_pages(k, v, table, torch.tensor([n], dtype=torch.int32, device=DEV), keep).tolist() == [n - 3]
+    assert torch.equal(flat(k)[:n - 3], want[0]) and torch.equal(flat(v)[:n - 3], want[1])
+
+
 def test_nothing_to_compact():
     k, v = (torch.randn(1, 4, 1, PAGE, D, device=DEV).bfloat16() for _ in range(2))
     i32 = dict(dtype=torch.int32, device=DEV)
