@@ -29,9 +29,8 @@ __device__ __forceinline__ int kperm(int rho) {  // S^T row rho -> key within th
   return 16 * s + 8 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
 }
 
-constexpr int NW = 4, ROWS = 32;
+constexpr int ROWS = 32;
 constexpr int PG = PAGE * HD;                    // numbers of a page's K (V)
-constexpr int KST = 3;                           // stages of K in a tile (V: two)
 
 struct Args {
   const bf16 *q, *kc, *vc;
@@ -181,15 +180,20 @@ __device__ __forceinline__ bf16x8 read_v8(const bf16* p) {
 }
 
 // ---- up to 128 pairs ----
-// A wavefront has 32 pairs, a workgroup's four share the pages: K and V of a page come by LDS DMA, two stages each, and a
-// page's exponentials run between the products of the page before with V, as in flash_prefill2_kernel (whose layouts these
-// are).  P is rounded to bf16 for the product (relative 2^-9: what a value's weight is off by); scores, maxima, sums and O
-// are fp32.
-__device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh, bf16* lds, int w, int lane) {
+// Four wavefronts have 32 pairs each and share the pages; with KG = 2 four more have the same pairs and every other page (two
+// pages of a workgroup on its way, one result of them: half the results of two workgroups).  K and V of a page come by LDS DMA,
+// two stages each, and a page's exponentials run between the products of the page before with V, as in flash_prefill2_kernel
+// (whose layouts these are).  P is rounded to bf16 for the product (relative 2^-9: what a value's weight is off by); scores,
+// maxima, sums and O are fp32.
+template <int KG>
+__device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh, bf16* lds_all, float2* sml, int wave, int lane) {
+  constexpr int CW = 4, CP = 16 / CW;                       // wavefronts that copy a page together, copies of each
+  const int w = wave % CW, kg = wave / CW;                  // pairs 32 w .., pages first + kg, first + kg + KG, ..
+  bf16* lds = lds_all + kg * (4 * PG);                      // K, K, V, V
   const int r32 = lane & 31, hh = lane >> 5;
   const Share S = share_of(W, most_of(A, W, lane));
   const int pairs = W.n * A.G, mine = w * 32 + r32, pair = min(mine, pairs - 1), row = W.row0 + pair / A.G;
-  const int lim = min(A.ctx_lens[row], A.max_ctx), least = least_of(lim);
+  const int lim = min(min(A.ctx_lens[row], A.max_ctx), S.end * PAGE), least = least_of(lim);
   f32x16 o[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -200,37 +204,39 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
     const table_t btr = table_of(A, W);
     // an instruction takes four rows of 256 bytes; rows past the last key (whatever they hold) are that key's again
-    constexpr int CP = 16 / NW;
     const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds)) + w * 1024;
     const int cr = 4 * w + (lane >> 4), cp = lane & 15;
     unsigned koff[CP], voff[CP];
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
-      const int r = cr + 4 * NW * i;
+      const int r = cr + 4 * CW * i;
       koff[i] = r * (HD * 2) + ((cp ^ (r & 15)) << 4);
       voff[i] = r * (HD * 2) + ((cp ^ (4 * (r & 3))) << 4);
     }
     auto copy = [&](const bf16* pool, int kt, int page, unsigned dst, const unsigned (&off)[CP]) {
       const bf16* from = pool + (size_t)page * page_sz + head_off;
-      const int top = S.last - kt * PAGE;
+      const int top = S.last - min(kt, S.end - 1) * PAGE;
       if (top >= PAGE - 1) {
 #pragma unroll
-        for (int i = 0; i < CP; ++i) ldsp::dma_lds16(from, off[i], dst + i * NW * 1024);
+        for (int i = 0; i < CP; ++i) ldsp::dma_lds16(from, off[i], dst + i * CW * 1024);
       } else {
 #pragma unroll
         for (int i = 0; i < CP; ++i)
-          ldsp::dma_lds16(from, off[i] - max(cr + 4 * NW * i - top, 0) * (HD * 2), dst + i * NW * 1024);
+          ldsp::dma_lds16(from, off[i] - max(cr + 4 * CW * i - top, 0) * (HD * 2), dst + i * CW * 1024);
       }
     };
-    auto copy_k = [&](int kt, int page, int stage) { copy(A.kc, kt, page, l0 + stage * (PG * 2), koff); };
-    auto copy_v = [&](int kt, int page) { copy(A.vc, kt, page, l0 + (KST + ((kt - S.first) & 1)) * (PG * 2), voff); };
-    auto page_of = [&](int kt) { return page_at(A, btr, min(kt, S.end - 1)); };
-    int p0 = page_of(S.first), p1 = page_of(S.first + 1), p2 = page_of(S.first + 2);   // pages kt, kt + 1, kt + 2
-    int kst = 0, flip = PG * 2;                                                        // stage of K; from this of V to the other
+    // (a group's last turn may be a page past the end: that is the last page again, of which it sees no key)
+    const int turns = (S.end - S.first + KG - 1) / KG;
+    auto page_of = [&](int t) { return page_at(A, btr, min(S.first + KG * t + kg, S.end - 1)); };
+    auto copy_k = [&](int t, int page) { copy(A.kc, S.first + KG * t + kg, page, l0 + (t & 1) * (PG * 2), koff); };
+    auto copy_v = [&](int t, int page) { copy(A.vc, S.first + KG * t + kg, page, l0 + (2 + (t & 1)) * (PG * 2), voff); };
+    int p0 = page_of(0), p1 = page_of(1);   // pages of this turn and the next
+    int flip = PG * 2;                      // from this turn's stage to the other
     bf16x8 qf[8];
     load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
-    copy_k(S.first, p0, 0);
-    if (S.first + 1 < S.end) copy_k(S.first + 1, p1, 1);
+    copy_k(0, p0);
+    copy_v(0, p0);
+    if (turns > 1) copy_k(1, p1);
 
     // places of this lane in a stage: K rows kperm(r32) (and 32 further), V as read_v8 takes it
     const int krow = kperm(r32), L = lane & 15;
@@ -239,7 +245,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     for (int s = 0; s < 8; ++s) kat[s] = (krow * HD + (((2 * s + hh) ^ (krow & 15)) << 3)) * 2;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
-      vat[db] = (KST * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1) +
+      vat[db] = (2 * PG + (8 * hh + (L >> 2)) * HD + 4 * (L & 1) +
                  ((((db ^ (L >> 2)) << 2) | (2 * ((lane >> 4) & 1) + ((L >> 1) & 1))) << 3)) * 2;
     const char* at_lds = reinterpret_cast<const char*>(lds);
     f32x16 sc[2];
@@ -264,25 +270,26 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         }
       }
 #pragma unroll
-      for (int db = 0; db < 4; ++db) vat[db] += flip;
-      flip = -flip;
+      for (int db = 0; db < 4; ++db) vat[db] += flip;   // (first_product has turned it round once more)
     };
-    // S^T = K . Q^T of page kt, two halves of 32 keys; the copies of its V and of the next K go out first
-    auto first_product = [&](int kt) {
-      // K of this page and V of the one before have landed; every wave is past the last page's K and the V before it
-      // (behind them the next K's copies, where there is one)
-      if (kt + 1 < S.end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CP) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // S^T = K . Q^T of turn t's page, two halves of 32 keys; the copies of its V and of the next K go out first
+    auto first_product = [&](int t) {
+      // K of this page and V of the one before have landed (at first: behind that K the first V and the next K); every wave is
+      // past the last page's K and the V before it
+      if (t > 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else if (turns > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * CP) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CP) : "memory");
       __syncthreads();
-      copy_v(kt, p0);
-      if (kt + 2 < S.end) copy_k(kt + 2, p2, kst == 0 ? KST - 1 : kst - 1);
+      if (t > 0) {
+        copy_v(t, p0);
+        if (t + 1 < turns) copy_k(t + 1, p1);
+      }
       p0 = p1;
-      p1 = p2;
-      p2 = page_of(kt + 3);
+      p1 = page_of(t + 2);
       bf16x8 kf[2][2];
       auto read_k2 = [&](int s) {
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = *reinterpret_cast<const bf16x8*>(at_lds + (kat[s] + kst * (PG * 2)) + 32 * kh * HD * 2);
+        for (int kh = 0; kh < 2; ++kh) kf[s & 1][kh] = *reinterpret_cast<const bf16x8*>(at_lds + kat[s] + 32 * kh * HD * 2);
       };
       read_k2(0);
 #pragma unroll
@@ -293,10 +300,12 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         for (int kh = 0; kh < 2; ++kh)
           sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s & 1][kh], qf[s], s == 0 ? f32x16{} : sc[kh], 0, 0, 0);
       }
-      kst = kst == KST - 1 ? 0 : kst + 1;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) kat[s] += flip;
+      flip = -flip;
       // Keys of register rr of half kh: 16 (rr >> 3) + 8 hh + (rr & 7)
-      const int left = lim - kt * PAGE - 8 * hh;
-      if (kt * PAGE + PAGE > least) {
+      const int k0 = (S.first + KG * t + kg) * PAGE, left = lim - k0 - 8 * hh;
+      if (k0 + PAGE > least) {
         asm volatile("");   // (a branch, not selects on every page)
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh)
@@ -349,13 +358,13 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         pf[i >> 1][i & 1] = __builtin_bit_cast(bf16x8, u32x4{pn[i][0], pn[i][1], pn[i][2], pn[i][3]});
       }
     };
-    first_product(S.first);
+    first_product(0);
     maxima();
 #pragma unroll
     for (int j = 0; j < 16; ++j) exps(j);
     take();
-    for (int kt = S.first + 1; kt < S.end; ++kt) {
-      first_product(kt);
+    for (int t = 1; t < turns; ++t) {
+      first_product(t);
       const int rescale = maxima();
       second_product(exps);
       take();
@@ -370,48 +379,65 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
-  float* so = reinterpret_cast<float*>(lds) + w * (32 * HD);   // the wavefront's rows, to be written whole
-  if (A.whole) {
-    put_rows(so, o, r32, hh);
-    __builtin_amdgcn_wave_barrier();
-    unsigned bad = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int p = 2 * i + hh;
-      const float den = __shfl(l, p, 64);
-      if (w * 32 + p < pairs) bad |= (unsigned)put_result(A, W, kvh, w * 32 + p, get_row(so, p, r32), den, r32) << i;
-    }
-    if (__any(bad)) {
-      for (int p = 0; p < 32; ++p)
-        if ((__ballot(bad >> (p / 2) & 1) >> (32 * (p & 1))) & 0xffffffffull) put_exact(A, W, kvh, w * 32 + p, lane);
-    }
+  const long to = mine >= pairs ? -1 : A.whole ? 0 : part_at(A, W, kvh, mine);
+  m = m == -INFINITY ? m : m * A.scale_log2;
+  if (!A.whole && S.first >= S.end) {   // a part of no page has its maximum only
+    if (kg == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(m, l);
     return;
   }
-  const long to = mine < pairs ? part_at(A, W, kvh, mine) : -1;
-  if (hh == 0 && to >= 0) A.part_ml[to] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
-  if (S.first >= S.end) return;   // (a part of no page has its maximum only)
-  put_rows(so, o, r32, hh);
-  __builtin_amdgcn_wave_barrier();
+  // the wavefront's rows to LDS and from there in whole rows, of both page groups: 32 / KG pairs for a wavefront
+  float* so = reinterpret_cast<float*>(lds_all);
+  put_rows(so + wave * (32 * HD), o, r32, hh);
+  if constexpr (KG > 1) {
+    if (hh == 0) sml[wave * 32 + r32] = make_float2(m, l);
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_wave_barrier();
+  }
+  unsigned bad = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const long at = __shfl(to, 2 * i + hh, 64);
-    if (at >= 0) *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = get_row(so, 2 * i + hh, r32);
+  for (int i = 0; i < 16 / KG; ++i) {
+    const int p = kg * (32 / KG) + 2 * i + hh;
+    const long at = __shfl(to, p, 64);
+    f32x4 sum = get_row(so + w * (32 * HD), p, r32);
+    float M = __shfl(m, p, 64), den = __shfl(l, p, 64);
+    if constexpr (KG > 1) {
+      const float2 a = sml[w * 32 + p], b = sml[(CW + w) * 32 + p];
+      M = fmaxf(a.x, b.x);
+      const float ea = a.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.x - M);
+      const float eb = b.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(b.x - M);
+      sum = sum * ea + get_row(so + (CW + w) * (32 * HD), p, r32) * eb;
+      den = fmaf(ea, a.y, eb * b.y);
+    }
+    if (at < 0) continue;
+    if (A.whole) {
+      bad |= (unsigned)put_result(A, W, kvh, w * 32 + p, sum, den, r32) << i;
+      continue;
+    }
+    *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = sum;
+    if (r32 == 0) A.part_ml[at] = make_float2(M, den);
+  }
+  if (__any(bad)) {
+    for (int i = 0; i < 32 / KG; ++i)
+      if ((__ballot(bad >> (i / 2) & 1) >> (32 * (i & 1))) & 0xffffffffull)
+        put_exact(A, W, kvh, w * 32 + kg * (32 / KG) + i, lane);
   }
 }
 
 // ---- up to 32 pairs ----
-// Four wavefronts, each with its own 32 keys at a time against the same pairs.  K and V come by LDS DMA into the wavefront's
-// own LDS, the next K while this one's weights are formed, the next V behind the second product; no barrier until the four
-// meet at the end.
+// NW wavefronts, each with its own 32 keys at a time against the same pairs.  K and V come by LDS DMA into the wavefront's
+// own LDS, the next K while this one's weights are formed, the next V behind the second product; no barrier until they meet at
+// the end.
 constexpr int KT = 32;
 
+template <int NW>
 __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, int w, int lane) {
   bf16* lds = lds_all + w * (2 * KT * HD);   // K and V; O at the end
   const int r32 = lane & 31, hh = lane >> 5;
   const int pairs = W.n * A.G, pair = min(r32, pairs - 1), row = W.row0 + pair / A.G;
   const int lim = min(A.ctx_lens[row], A.max_ctx), least = least_of(lim);
   const Share S = share_of(W, most_of(A, W, lane));
-  const int u0 = S.first * 2 + w, u1 = S.first < S.end ? S.last / KT + 1 : 0;   // units of 32 keys, this wavefront's every fourth
+  const int u0 = S.first * 2 + w, u1 = S.first < S.end ? S.last / KT + 1 : 0;   // units of 32 keys, every NW-th for this wavefront
 
   const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
   const table_t btr = table_of(A, W);
@@ -522,7 +548,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     if (w == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(-INFINITY, 0.f);
     return;
   }
-  // the four meet: first their maxima and sums (where all wavefronts' copies have been), then O in their place
+  // they meet: first their maxima and sums (where all wavefronts' copies have been), then O in their place
   constexpr int EACH = ROWS * 32 / (NW * 64);   // 16-byte pieces of a thread
   float2* sml = reinterpret_cast<float2*>(lds_all);
   __syncthreads();
@@ -572,16 +598,19 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
   }
 }
 
+template <int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(
     Args A, const Work* __restrict__ works) {
-  static_assert(NW * 2 * KT <= (KST + 2) * PAGE, "few_role in the LDS of tile_role");
-  __shared__ __attribute__((aligned(16))) bf16 lds[(KST + 2) * PG];
+  constexpr int KG = NW / 4;
+  static_assert(NW * 2 * KT * HD == KG * 4 * PG, "both roles in the same LDS");
+  __shared__ __attribute__((aligned(16))) bf16 lds[KG * 4 * PG];
+  __shared__ float2 sml[KG > 1 ? NW * 32 : 1];
   // heads first: with 8 kv heads an XCD has one of them, and its L2 that head's pages for all tiles
   const int b = blockIdx.x;
   const Work W = works[b / A.Hkv];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (W.n * A.G > ROWS) tile_role(A, W, b % A.Hkv, lds, w, lane);
-  else few_role(A, W, b % A.Hkv, lds, w, lane);
+  if (W.n * A.G > ROWS) tile_role<KG>(A, W, b % A.Hkv, lds, sml, w, lane);
+  else few_role<NW>(A, W, b % A.Hkv, lds, w, lane);
 }
 
 // The parts of a (row, head) pair: GROUPS half wavefronts, four numbers per lane, each with every GROUPS-th part.  A group has
@@ -673,14 +702,15 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* 
 // tables; part_o, part_ml: base[R] * Hq * (128 | 2) floats.  Every part of every row belongs to one work.
 P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int num_pages,
                                  const int* block_tables, int bt_stride, const int* ctx_lens, int max_ctx, const int* works,
-                                 int n_works, const int* base, const int* tables, int R, int parts, int even, int Hq, int Hkv,
+                                 int n_works, int waves, const int* base, const int* tables, int R, int parts, int even, int Hq, int Hkv,
                                  int head_dim, float scale, void* out, int ldo, float* part_o, float* part_ml, hipStream_t stream) {
   if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0) return (int)hipErrorInvalidValue;
   const float sl2 = scale * 1.4426950408889634f;
   const int G = Hq / Hkv;
   const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, base, part_o,
                   (float2*)part_ml, (bf16*)out, ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G, parts == R, sl2};
-  hipLaunchKernelGGL(prefix_attn_kernel, dim3(n_works * Hkv), dim3(NW * 64), 0, stream, A, (const Work*)works);
+  if (waves == 8) hipLaunchKernelGGL(prefix_attn_kernel<8>, dim3(n_works * Hkv), dim3(512), 0, stream, A, (const Work*)works);
+  else hipLaunchKernelGGL(prefix_attn_kernel<4>, dim3(n_works * Hkv), dim3(256), 0, stream, A, (const Work*)works);
   if (int e = (int)hipGetLastError()) return e;
   if (parts == R) return 0;
   if (parts > 8 * R)

@@ -31,6 +31,7 @@ class PrefixPlan:
     n_kv: int
     max_ctx: int
     tables: int            # block tables it reads
+    waves: int             # wavefronts of a workgroup, 4 or 8
     even: int              # results of every row, where they are equally many (else 0)
     parts: int             # results of parts, over all rows
     works: torch.Tensor    # int32 [n, 8]
@@ -93,12 +94,13 @@ class _Shape:
                 count[a:a + n] = [count[a] + C] * n
         return works, count
 
-    def micros(self, share: bool, shared_parts: int, own_parts: int) -> float:
-        """About how long a call takes: a launch and its first loads 4.5 us; a page of a tile of 128 pairs 1.35 us where CUs have
-        one, 2.1 for two together; 32 keys of a wavefront 0.75; bytes at 5 TB/s from memory, 15 from L2; a second launch 2.5,
-        the parts' results 0.5 us per MB, written and read, and 150 ns per 1000 of them brought together.  Over 56 batches of 2
-        to 768 rows behind 128 to 32768 tokens, the cut that it puts first takes 2.4 % longer than the fastest one on average
-        (512 and 1024 workgroups whatever the batch: 29 %)."""
+    def micros(self, waves: int, share: bool, shared_parts: int, own_parts: int) -> float:
+        """About how long a call takes: constants fitted to timings of 78 batches, of 2 to 768 rows behind 128 to 32768 tokens, cut
+        in all ways.  A launch and its first loads 3.2 us (of 8 wavefronts 4.6); a page of a tile of 128 pairs 1.2 us where CUs
+        have one workgroup, 1.4 where they have two, two pages of 8 wavefronts 2.1; 32 keys of a wavefront 1.05 (1.2); what memory
+        and L2 add, as if they were three sides of a box, at 8.5 and 24 TB/s; a second launch 4.5, 0.6 per MB of the parts'
+        results, and 0.08 for every part of a row.  The cut that it puts first takes 2.9 % longer than the fastest one on average
+        (with 4 wavefronts only: 5.7 %)."""
         many = few = many_pages = few_units = parts = read = loaded = 0
         for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
             own = (self.pages - p + 1) // 2       # (contexts end somewhere up to the plan's longest)
@@ -119,19 +121,27 @@ class _Shape:
                 else:
                     few += n * C * self.n_kv
                     few_units = max(few_units, -(-pages // (2 * C)))
-        page = self.n_kv * 32768e-6                # MB
-        t_many = many_pages * (1.35 if many <= 256 else 2.1 * max(1.0, many / 512))
-        t_few = few_units * 0.75 * max(1.0, few / 512)
-        t = max(t_many, t_few) if many + few <= 512 else t_many + t_few
-        t = 4.5 + math.hypot(t, read * page / 5, loaded * page / 15)
+        eight, most = waves == 8, 2048 // waves        # (workgroups at once)
+        if eight:
+            many_pages, few_units = -(-many_pages // 2), -(-few_units // 2)
+        t_many = many_pages * (2.1 if eight else 1.2 if many <= 256 else 1.4) * max(1.0, many / most)
+        t_few = few_units * (1.2 if eight else 1.05) * max(1.0, few / most)
+        t = max(t_many, t_few) if many + few <= most else t_many + t_few
+        page = self.n_kv * 32768e-6                    # MB
+        t = (4.6 if eight else 3.2) + math.hypot(t, read * page / 8.5, loaded * page / 24)
         if parts > self.R:
-            t += 2.5 + 0.5e-6 * parts * self.n_heads * 512 + 1.5e-4 * self.R * self.n_heads
+            t += 4.5 + 0.6e-6 * parts * self.n_heads * 512 + 0.08 * parts / self.R
         return t
 
     def choose(self):
-        ways = [(False, 1, own) for own in OWN_PARTS]
-        if any(p for p, _t, _r in self.groups):
-            ways += [(True, shared, own) for shared in SHARED_PARTS for own in OWN_PARTS]
+        """The way (wavefronts of a workgroup, shared or alone, parts of shared pages, parts of a sequence's own) to cut it."""
+        upto = lambda parts, pages: [c for c in parts if c == 1 or c <= -(-pages // 2)]
+        most = max(p for p, _t, _r in self.groups)
+        least = min(p for p, _t, _r in self.groups)
+        ways = [(waves, False, 1, own) for waves in (4, 8) for own in upto(OWN_PARTS, self.pages)]
+        if most:
+            ways += [(waves, True, shared, own) for waves in (4, 8) for shared in upto(SHARED_PARTS, most)
+                     for own in upto(OWN_PARTS, self.pages - least)]
         return min(ways, key=lambda way: self.micros(*way))
 
 
@@ -160,7 +170,8 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
         raise ValueError("prefix_plan: seqs must give a block table (0 ..) to each of the %d rows" % R)
 
     shape = _Shape(groups, seqs, n_heads, n_kv, max_ctx)
-    works, count = shape.works(*shape.choose())
+    waves, *way = shape.choose()
+    works, count = shape.works(*way)
     base = [0]
     for n in count:
         base.append(base[-1] + n)
@@ -169,7 +180,7 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     flat = torch.tensor(flat, dtype=torch.int32).to(dev)
     n = 8 * len(works)
     even = count[0] if min(count) == max(count) else 0
-    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, even, base[-1], flat[:n].view(-1, 8), flat[n + R:],
+    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, waves, even, base[-1], flat[:n].view(-1, 8), flat[n + R:],
                       flat[n:n + R])
 
 
@@ -261,7 +272,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     with _lib.device_of(dev):
         _lib.check(_lib.lib().p2p_prefix_attention(
             q.data_ptr(), q.stride(0), kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(),
-            plan.max_ctx, works.data_ptr(), works.shape[0], plan.base.data_ptr(), plan.row_tables.data_ptr(), R, plan.parts, plan.even,
+            plan.max_ctx, works.data_ptr(), works.shape[0], plan.waves, plan.base.data_ptr(), plan.row_tables.data_ptr(), R, plan.parts, plan.even,
             n_heads, n_kv, HEAD_DIM, scale, out.data_ptr(), out.stride(0), po.data_ptr(), pml.data_ptr(),
             torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
     return out

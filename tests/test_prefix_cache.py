@@ -28,7 +28,7 @@ def test_plans_that_are_refused(why, call):
         call()
 
 
-@pytest.mark.parametrize("way", [None, (True, 1, 1), (True, 3, 1), (True, 48, 8), (False, 1, 1), (False, 1, 16)])
+@pytest.mark.parametrize("way", [None, (4, True, 1, 1), (8, True, 3, 1), (4, True, 48, 8), (8, False, 1, 1), (4, False, 1, 16)])
 def test_whatever_the_cut_every_key_of_a_row_is_in_one_part(way, monkeypatch):
     """way: the cut (None: the one that the plan chooses)."""
     if way is not None:

@@ -60,8 +60,8 @@ def _run(q, k, v, table, ctx, plan, **kw):
     return ops.prefix_attention(q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), ctx.to(DEV), plan, **kw)
 
 
-# cuts of a batch (shared pages or not, parts of them, parts of a sequence's own pages); None: the one that the plan chooses
-WAYS = [None, (True, 1, 1), (True, 5, 2), (False, 1, 1), (False, 1, 3)]
+# cuts of a batch (wavefronts of a workgroup, shared pages or not, parts of them, parts of a sequence's own pages); None: the one that the plan chooses
+WAYS = [None, (4, True, 1, 1), (8, True, 1, 1), (4, True, 5, 2), (8, True, 3, 1), (4, False, 1, 1), (8, False, 1, 1), (4, False, 1, 3)]
 
 
 @pytest.fixture(params=WAYS, ids=str)
@@ -87,7 +87,7 @@ def test_prefix_attention_of_decode_rows(way, Hq, Hkv, groups, own):
 @pytest.mark.parametrize("groups,own", [([(2, 560)], 9), ([(40, 150)], 3), ([(1, 0), (2, 700)], 2)])
 def test_prefix_attention_in_many_parts(groups, own, monkeypatch):
     """One kv head: up to some 300 parts of a row."""
-    monkeypatch.setattr(prefix._Shape, "choose", lambda self: (True, 400, 100))
+    monkeypatch.setattr(prefix._Shape, "choose", lambda self: (4, True, 400, 100))
     q, k, v, table, seqs, ctx, rows, most = _batch(groups, 8, 1, own, own)
     plan = ops.prefix_plan(rows, 8, 1, most, DEV)
     want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 1, 1 / math.sqrt(D), most)
