@@ -37,6 +37,12 @@ class PrefixPlan:
     works: torch.Tensor    # int32 [n, 8]
     base: torch.Tensor     # int32 [rows + 1]: parts of the rows before
     row_tables: torch.Tensor   # int32 [rows]
+    launch: tuple = dataclasses.field(init=False, repr=False, compare=False)   # what every call hands on of it
+
+    def __post_init__(self):
+        object.__setattr__(self, "launch", (
+            self.works.data_ptr(), self.works.shape[0], self.waves, self.base.data_ptr(), self.row_tables.data_ptr(), self.rows,
+            self.parts, self.even, self.n_heads, self.n_kv, HEAD_DIM))
 
 
 def _int(x, what: str) -> int:
@@ -184,12 +190,10 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
                       flat[n:n + R])
 
 
-def prefix_workspace(plan: PrefixPlan) -> tuple:
-    """(parts' outputs, parts' maxima and sums) for :func:`prefix_attention`; a launch uses them until it ends, so calls
-    that may run at once (on several streams, in several graphs) take one each."""
-    dev = plan.works.device
-    return (torch.empty(plan.parts * plan.n_heads * HEAD_DIM, device=dev, dtype=torch.float32),
-            torch.empty(plan.parts * plan.n_heads * 2, device=dev, dtype=torch.float32))
+def prefix_workspace(plan: PrefixPlan) -> torch.Tensor:
+    """The parts' outputs, maxima and sums for :func:`prefix_attention`, fp32; a call uses them until it ends, so calls that may
+    run at once (on several streams, in several graphs) take one each."""
+    return torch.empty(plan.parts * plan.n_heads * (HEAD_DIM + 2), device=plan.works.device, dtype=torch.float32)
 
 
 def _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale):
@@ -213,17 +217,17 @@ def _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, s
     need(0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
     need(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width and out.stride(1) == 1,
          "out must be bf16 [%d or more, %d], rows contiguous" % (R, width))
-    need(all(t.device == q.device for t in (k_cache, v_cache, block_tables, ctx_lens, plan.works, out) + workspace),
+    need(all(t.device == q.device for t in (k_cache, v_cache, block_tables, ctx_lens, plan.works, out)),
          "tensors and plan must be on one device")
-    need(not workspace or all(w.dtype == torch.float32 and w.is_contiguous() for w in workspace), "workspace is not this plan's")
-    need(not workspace or (workspace[0].numel() >= plan.parts * width and workspace[1].numel() >= plan.parts * n_heads * 2),
-         "workspace is not this plan's")
+    need(workspace is None or (workspace.device == q.device and workspace.dtype == torch.float32 and workspace.is_contiguous()
+                               and workspace.numel() >= plan.parts * n_heads * (HEAD_DIM + 2)
+                               and workspace.data_ptr() % 16 == 0), "workspace is not this plan's (prefix_workspace)")
     raise AssertionError("prefix_attention: the two forms of its conditions differ")
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                      ctx_lens: torch.Tensor, plan: PrefixPlan, out: torch.Tensor | None = None,
-                     workspace: tuple | None = None, scale: float | None = None) -> torch.Tensor:
+                     workspace: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """q: [R, n_heads * 128] bf16 -> out [R, n_heads * 128] bf16, as :func:`paged_attention` with the plan's tables.
 
     Row r attends the first ``min(ctx_lens[r], plan.max_ctx)`` tokens of its block table; a row that sees none is 0.  Rows
@@ -234,10 +238,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if scale is None:
         scale = SCALE
     if out is None:
-        out = torch.empty(q.shape[0], width, device=q.device, dtype=torch.bfloat16)
-    dev = q.get_device()     # (-1: CPU)
-    if workspace is None:
-        workspace = prefix_workspace(plan) if dev >= 0 and plan.works.get_device() == dev else ()
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dev = q.get_device()     # (-1: not a GPU's)
+    if workspace is None and dev >= 0:
+        workspace = prefix_workspace(plan)
     works = plan.works
     try:
         Rq, wq = q.shape
@@ -252,27 +256,29 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
               and q.stride(1) == out.stride(1) == block_tables.stride(1) == ctx_lens.stride(0) == 1
               and k_cache.is_contiguous() and v_cache.is_contiguous() and 0 < scale < math.inf
               and dev == out.get_device() == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
-              == ctx_lens.get_device() == works.get_device() and q.device.type == k_cache.device.type == ctx_lens.device.type)
+              == ctx_lens.get_device() == works.get_device())
         kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
         if ok and dev >= 0:
-            po, pml = workspace
-            ok = ((kp | vp) % 16 == 0 and po.get_device() == pml.get_device() == dev and po.dtype == pml.dtype == torch.float32
-                  and po.is_contiguous() and pml.is_contiguous() and po.numel() >= plan.parts * width
-                  and pml.numel() >= plan.parts * n_heads * 2)
+            wp = workspace.data_ptr()
+            ok = ((kp | vp | wp) % 16 == 0 and workspace.get_device() == dev and workspace.dtype == torch.float32
+                  and workspace.is_contiguous() and workspace.numel() >= plan.parts * n_heads * (HEAD_DIM + 2))
+        elif ok:
+            ok = all(t.device.type == "cpu" for t in (q, k_cache, v_cache, block_tables, ctx_lens, works, out))
     except ValueError:       # another number of dimensions
         ok = False
     if not ok:
-        _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, tuple(workspace), scale)
+        _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale)
     if dev < 0:
         ctx = ctx_lens[:R].clamp(0, plan.max_ctx)
         paged_attention_ref(q[:R], k_cache, v_cache, block_tables, plan.row_tables, ctx.clamp(min=1), n_heads, n_kv, scale,
                             out[:R])
         out[:R] = torch.where((ctx > 0)[:, None], out[:R], 0)
         return out
-    with _lib.device_of(dev):
-        _lib.check(_lib.lib().p2p_prefix_attention(
-            q.data_ptr(), q.stride(0), kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(),
-            plan.max_ctx, works.data_ptr(), works.shape[0], plan.waves, plan.base.data_ptr(), plan.row_tables.data_ptr(), R, plan.parts, plan.even,
-            n_heads, n_kv, HEAD_DIM, scale, out.data_ptr(), out.stride(0), po.data_ptr(), pml.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return prefix_attention(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale)
+    _lib.check(_lib.lib().p2p_prefix_attention(
+        q.data_ptr(), q.stride(0), kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx,
+        *plan.launch, scale, out.data_ptr(), out.stride(0), wp, wp + plan.parts * width * 4,
+        torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
     return out
