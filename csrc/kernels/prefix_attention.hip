@@ -20,7 +20,7 @@ struct Work {
   int row0, n;         // query rows
   int table;           // block-table row whose pages they read
   int page0, page1;    // pages
-  int part, of;        // this is part `part` of `of` equal ones of the pages that some row sees
+  int part, of;        // this is part `part` of `of` equal ones of the pages that some row sees (of 0: these are the part's pages)
   int slot;            // and part slot + part of its rows' results
 };
 
@@ -39,7 +39,7 @@ struct Args {
   float2* part_ml;
   bf16* out;
   int ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G;
-  int whole;             // every row has one part, which is its result
+  int even;              // parts of every row, where they are equally many (1: the results themselves), else 0
   float scale_log2;
 };
 
@@ -48,6 +48,7 @@ struct Share {
   int first, end, last;
 };
 __device__ __forceinline__ Share share_of(const Work& W, int most) {
+  if (W.of == 0) return {W.page0, W.page1, W.page1 * PAGE - 1};   // (known before the context lengths have come)
   const int np = max(0, (min(most, W.page1 * PAGE) + PAGE - 1) / PAGE - W.page0);
   const int first = W.page0 + (int)((long)np * W.part / W.of), end = W.page0 + (int)((long)np * (W.part + 1) / W.of);
   return {first, end, min(most, end * PAGE) - 1};
@@ -64,14 +65,14 @@ __device__ __forceinline__ int least_of(int lim) {   // of the wavefront's 32 ro
   for (int o = 16; o > 0; o >>= 1) lim = min(lim, __shfl_xor(lim, o, 64));
   return __builtin_amdgcn_readfirstlane(lim);
 }
-// Block tables through scalar loads: a vector load's wait would be one for the copies in flight, too.
-typedef const __attribute__((address_space(4))) int* table_t;
-__device__ __forceinline__ table_t table_of(const Args& A, const Work& W) {
-  return (table_t)(uintptr_t)(A.bt + (size_t)W.table * A.bt_stride);
-}
-__device__ __forceinline__ int page_at(const Args& A, table_t btr, int at) {
-  return min(max(btr[at], 0), A.num_pages - 1);
-}
+// A work's page numbers, through scalar loads: a vector load's wait would be one for the copies in flight, too.
+struct Pages {
+  const __attribute__((address_space(4))) int* row;
+  int num_pages;
+  __device__ __forceinline__ Pages(const Args& A, const Work& W)
+      : row((const __attribute__((address_space(4))) int*)(uintptr_t)(A.bt + (size_t)W.table * A.bt_stride)), num_pages(A.num_pages) {}
+  __device__ __forceinline__ int operator()(int at) const { return min(max(row[at], 0), num_pages - 1); }
+};
 
 __device__ __forceinline__ float max_of_halves(float x) {   // of lanes i and i + 32
   const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -102,7 +103,8 @@ __device__ __forceinline__ f32x4 get_row(const float* so, int pair, int piece) {
 
 // where a pair's result of this part belongs
 __device__ __forceinline__ long part_at(const Args& A, const Work& W, int kvh, int pair) {
-  return ((long)(A.base[W.row0 + pair / A.G] + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
+  const int row = W.row0 + pair / A.G, before = A.even ? row * A.even : A.base[row];
+  return ((long)(before + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
 }
 
 // One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
@@ -147,12 +149,12 @@ __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINI
 
 // Result of pair `pair` from its only part: lane r32 has numbers 4 r32 ..  A bit of `bad` says that it has to be done again.
 __device__ __forceinline__ bool put_result(const Args& A, const Work& W, int kvh, int pair, f32x4 sum, float den, int r32) {
-  const float by = den == 0.f ? 0.f : 1.f / den;   // (0: no key)
+  const float by = 1.f / den;
   bf16x4 y;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = sum[i] * by;
+    const float x = den == 0.f ? 0.f : sum[i] * by;   // (no key, whatever the values of others are)
     bad |= not_finite(x);
     y[i] = f2bf(x);
   }
@@ -191,7 +193,8 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
   const int w = wave % CW, kg = wave / CW;                  // pairs 32 w .., pages first + kg, first + kg + KG, ..
   bf16* lds = lds_all + kg * (4 * PG);                      // K, K, V, V
   const int r32 = lane & 31, hh = lane >> 5;
-  const Share S = share_of(W, most_of(A, W, lane));
+  const Pages pages(A, W);
+  const Share S = share_of(W, W.of ? most_of(A, W, lane) : 0);
   const int pairs = W.n * A.G, mine = w * 32 + r32, pair = min(mine, pairs - 1), row = W.row0 + pair / A.G;
   const int lim = min(min(A.ctx_lens[row], A.max_ctx), S.end * PAGE), least = least_of(lim);
   f32x16 o[4];
@@ -202,7 +205,6 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
   float m = -INFINITY, l = 0.f;
   if (S.first < S.end) {
     const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
-    const table_t btr = table_of(A, W);
     // an instruction takes four rows of 256 bytes; rows past the last key (whatever they hold) are that key's again
     const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds)) + w * 1024;
     const int cr = 4 * w + (lane >> 4), cp = lane & 15;
@@ -227,7 +229,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     };
     // (a group's last turn may be a page past the end: that is the last page again, of which it sees no key)
     const int turns = (S.end - S.first + KG - 1) / KG;
-    auto page_of = [&](int t) { return page_at(A, btr, min(S.first + KG * t + kg, S.end - 1)); };
+    auto page_of = [&](int t) { return pages(min(S.first + KG * t + kg, S.end - 1)); };
     auto copy_k = [&](int t, int page) { copy(A.kc, S.first + KG * t + kg, page, l0 + (t & 1) * (PG * 2), koff); };
     auto copy_v = [&](int t, int page) { copy(A.vc, S.first + KG * t + kg, page, l0 + (2 + (t & 1)) * (PG * 2), voff); };
     int p0 = page_of(0), p1 = page_of(1);   // pages of this turn and the next
@@ -379,9 +381,9 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
-  const long to = mine >= pairs ? -1 : A.whole ? 0 : part_at(A, W, kvh, mine);
+  const long to = mine >= pairs ? -1 : A.even == 1 ? 0 : part_at(A, W, kvh, mine);
   m = m == -INFINITY ? m : m * A.scale_log2;
-  if (!A.whole && S.first >= S.end) {   // a part of no page has its maximum only
+  if (!A.even == 1 && S.first >= S.end) {   // a part of no page has its maximum only
     if (kg == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(m, l);
     return;
   }
@@ -410,7 +412,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       den = fmaf(ea, a.y, eb * b.y);
     }
     if (at < 0) continue;
-    if (A.whole) {
+    if (A.even == 1) {
       bad |= (unsigned)put_result(A, W, kvh, w * 32 + p, sum, den, r32) << i;
       continue;
     }
@@ -434,13 +436,13 @@ template <int NW>
 __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, int w, int lane) {
   bf16* lds = lds_all + w * (2 * KT * HD);   // K and V; O at the end
   const int r32 = lane & 31, hh = lane >> 5;
+  const Pages pages(A, W);
   const int pairs = W.n * A.G, pair = min(r32, pairs - 1), row = W.row0 + pair / A.G;
   const int lim = min(A.ctx_lens[row], A.max_ctx), least = least_of(lim);
-  const Share S = share_of(W, most_of(A, W, lane));
+  const Share S = share_of(W, W.of ? most_of(A, W, lane) : 0);
   const int u0 = S.first * 2 + w, u1 = S.first < S.end ? S.last / KT + 1 : 0;   // units of 32 keys, every NW-th for this wavefront
 
   const size_t page_sz = (size_t)A.Hkv * PG, head_off = (size_t)kvh * PG;
-  const table_t btr = table_of(A, W);
   const unsigned l0 = __builtin_amdgcn_readfirstlane(ldsp::lds_off(lds));
   const int cr = lane >> 4, cp = lane & 15;
   auto copy = [&](const bf16* pool, int u, int page, bool is_v) {
@@ -453,7 +455,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
                       l0 + is_v * (KT * HD * 2) + i * 1024);
     }
   };
-  auto page_of = [&](int u) { return page_at(A, btr, min(u, u1 - 1) / 2); };
+  auto page_of = [&](int u) { return pages(min(u, u1 - 1) / 2); };
 
   bf16x8 qf[8];
   load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
@@ -543,8 +545,8 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     }
   }
   l += __shfl_xor(l, 32, 64);
-  const long to = r32 >= pairs ? -1 : A.whole ? 0 : part_at(A, W, kvh, r32);
-  if (!A.whole && S.first >= S.end) {   // a part of no page has its maximum only
+  const long to = r32 >= pairs ? -1 : A.even == 1 ? 0 : part_at(A, W, kvh, r32);
+  if (!A.even == 1 && S.first >= S.end) {   // a part of no page has its maximum only
     if (w == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(-INFINITY, 0.f);
     return;
   }
@@ -584,7 +586,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NW; ++x) sum += get_row(all + x * (KT * HD), p, r32) * weight[i][x];
-    if (A.whole) {
+    if (A.even == 1) {
       bad |= (unsigned)put_result(A, W, kvh, p, sum, den[i], r32) << i;
       continue;
     }
@@ -616,11 +618,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // The parts of a (row, head) pair: GROUPS half wavefronts, four numbers per lane, each with every GROUPS-th part.  A group has
 // the statistics and outputs of eight parts in flight together, what they weigh is known when they have come; groups meet in LDS.
 template <int GROUPS>
-__global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* __restrict__ tables, int R, int even) {
+__global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* __restrict__ tables, int R) {
   const int Hq = A.Hkv * A.G, lane = threadIdx.x & 63, r32 = lane & 31, g = GROUPS == 1 ? 0 : threadIdx.x >> 5;
   const int pair0 = GROUPS == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, pair = min(pair0, R * Hq - 1);
   const int r = pair / Hq, h = pair % Hq;
-  const int b0 = even ? r * even : A.base[r], n = even ? even : A.base[r + 1] - b0;
+  const int b0 = A.even ? r * A.even : A.base[r], n = A.even ? A.even : A.base[r + 1] - b0;
   const float2* ml = A.part_ml + (size_t)b0 * Hq + h;
   const float* po = A.part_o + ((size_t)b0 * Hq + h) * HD + 4 * r32;
   float M = -INFINITY, den = 0.f;
@@ -708,14 +710,14 @@ P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, co
   const float sl2 = scale * 1.4426950408889634f;
   const int G = Hq / Hkv;
   const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, base, part_o,
-                  (float2*)part_ml, (bf16*)out, ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G, parts == R, sl2};
+                  (float2*)part_ml, (bf16*)out, ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G, even, sl2};
   if (waves == 8) hipLaunchKernelGGL(prefix_attn_kernel<8>, dim3(n_works * Hkv), dim3(512), 0, stream, A, (const Work*)works);
   else hipLaunchKernelGGL(prefix_attn_kernel<4>, dim3(n_works * Hkv), dim3(256), 0, stream, A, (const Work*)works);
   if (int e = (int)hipGetLastError()) return e;
-  if (parts == R) return 0;
+  if (even == 1) return 0;
   if (parts > 8 * R)
-    hipLaunchKernelGGL(prefix_combine_kernel<8>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R, even);
+    hipLaunchKernelGGL(prefix_combine_kernel<8>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R);
   else
-    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 7) / 8), dim3(256), 0, stream, A, tables, R, even);
+    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 7) / 8), dim3(256), 0, stream, A, tables, R);
   P2P_CHECK_LAUNCH();
 }

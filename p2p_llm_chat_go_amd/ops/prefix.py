@@ -89,7 +89,7 @@ class _Shape:
         for p, tiles, _runs in self.groups:
             if share and p:
                 C = min(shared_parts, -(-p // 2))
-                works += [(a, n, t, 0, p, c, C, 0) for c in range(C) for a, n, t in tiles]
+                works += [(a, n, t, p * c // C, p * (c + 1) // C, c, 0, 0) for c in range(C) for a, n, t in tiles]
                 for a, n, _t in tiles:
                     count[a:a + n] = [C] * n
         for p, _tiles, runs in self.groups:
@@ -105,8 +105,8 @@ class _Shape:
         in all ways.  A launch and its first loads 3.2 us (of 8 wavefronts 4.6); a page of a tile of 128 pairs 1.2 us where CUs
         have one workgroup, 1.4 where they have two, two pages of 8 wavefronts 2.1; 32 keys of a wavefront 1.05 (1.2); what memory
         and L2 add, as if they were three sides of a box, at 8.5 and 24 TB/s; a second launch 4.5, 0.6 per MB of the parts'
-        results, and 0.08 for every part of a row.  The cut that it puts first takes 2.9 % longer than the fastest one on average
-        (with 4 wavefronts only: 5.7 %)."""
+        results, and 0.08 for every part of a row; rows alone in parts a tenth more than that.  The cut that it puts first takes
+        3.0 % longer than the fastest one on average (with 4 wavefronts only: 5.7 %)."""
         many = few = many_pages = few_units = parts = read = loaded = 0
         for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
             own = (self.pages - p + 1) // 2       # (contexts end somewhere up to the plan's longest)
@@ -137,6 +137,8 @@ class _Shape:
         t = (4.6 if eight else 3.2) + math.hypot(t, read * page / 8.5, loaded * page / 24)
         if parts > self.R:
             t += 4.5 + 0.6e-6 * parts * self.n_heads * 512 + 0.08 * parts / self.R
+            if not share:
+                t *= 1.1
         return t
 
     def choose(self):

@@ -58,11 +58,11 @@ def test_whatever_the_cut_every_key_of_a_row_is_in_one_part(way, monkeypatch):
             at += n
         ctx = [rng.choice([0, 1, 64, 100, 1900, most]) for _ in range(R)]
         for row0, n, table, p0, p1, part, of, slot in plan.works.tolist():
-            assert 1 <= n * (heads // kv) and 0 <= part < of
+            assert 1 <= n * (heads // kv) and (0 <= part < of or of == 0)
             seen = max(0, -(-min(max(ctx[row0:row0 + n]), p1 * PAGE) // PAGE) - p0)     # pages that some row sees
-            a, b = p0 + seen * part // of, p0 + seen * (part + 1) // of
+            a, b = (p0 + seen * part // of, p0 + seen * (part + 1) // of) if of else (p0, p1)
             for r in range(row0, row0 + n):
-                assert table == seqs[r] or (table == first[r] and p0 == 0)
+                assert table == seqs[r] or (table == first[r] and of == 0)
                 parts[r].append((slot + part, a, b))
         for r in range(R):
             got = sorted(parts[r])

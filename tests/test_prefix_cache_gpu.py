@@ -121,6 +121,21 @@ def test_rows_that_see_nothing_part_of_the_prefix_or_more_than_the_plan(way, Hq,
     assert bool((got[[0, 1, 24]] == 0).all())
 
 
+def test_rows_inside_their_shared_pages(way):
+    """Contexts that end in the shared pages, or before them; what none of the rows sees is nan."""
+    q, k, v, table, seqs, _ctx, rows, _most = _batch([(30, 4)], 8, 2, 1, 8)
+    ctx = torch.randint(0, 150, (30,), generator=torch.Generator().manual_seed(1)).int()
+    ctx[:4] = torch.tensor([0, 149, 64, 0])
+    for c in (k, v):
+        c[table[0, 3]] = NAN
+        c[table[0, 2], :, 149 - 128:] = NAN
+    plan = ops.prefix_plan(rows, 8, 2, 256, DEV)
+    want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 2, 1 / math.sqrt(D), 256)
+    _check(_run(q, k, v, table, ctx, plan), want, bound)
+    ctx.zero_()
+    assert bool((_run(q, k, v, table, ctx, plan) == 0).all())
+
+
 @pytest.mark.parametrize("tokens", [1, 20])
 def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(way, tokens):
     q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 3, tokens)
