@@ -71,7 +71,9 @@ struct Pages {
   int num_pages;
   __device__ __forceinline__ Pages(const Args& A, const Work& W)
       : row((const __attribute__((address_space(4))) int*)(uintptr_t)(A.bt + (size_t)W.table * A.bt_stride)), num_pages(A.num_pages) {}
-  __device__ __forceinline__ int operator()(int at) const { return min(max(row[at], 0), num_pages - 1); }
+  __device__ __forceinline__ int entry(int at) const { return row[at]; }
+  __device__ __forceinline__ int page(int entry) const { return min(max(entry, 0), num_pages - 1); }
+  __device__ __forceinline__ int operator()(int at) const { return page(entry(at)); }
 };
 
 __device__ __forceinline__ float max_of_halves(float x) {   // of lanes i and i + 32
@@ -229,16 +231,16 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     };
     // (a group's last turn may be a page past the end: that is the last page again, of which it sees no key)
     const int turns = (S.end - S.first + KG - 1) / KG;
-    auto page_of = [&](int t) { return pages(min(S.first + KG * t + kg, S.end - 1)); };
+    auto entry_of = [&](int t) { return pages.entry(min(S.first + KG * t + kg, S.end - 1)); };
     auto copy_k = [&](int t, int page) { copy(A.kc, S.first + KG * t + kg, page, l0 + (t & 1) * (PG * 2), koff); };
     auto copy_v = [&](int t, int page) { copy(A.vc, S.first + KG * t + kg, page, l0 + (2 + (t & 1)) * (PG * 2), voff); };
-    int p0 = page_of(0), p1 = page_of(1);   // pages of this turn and the next
+    int p0 = pages.page(entry_of(0)), p1 = entry_of(1);   // this turn's page, the next one's entry in the block table
     int flip = PG * 2;                      // from this turn's stage to the other
     bf16x8 qf[8];
     load_q(A, row, kvh * A.G + pair % A.G, hh, qf);
     copy_k(0, p0);
     copy_v(0, p0);
-    if (turns > 1) copy_k(1, p1);
+    if (turns > 1) copy_k(1, pages.page(p1));
 
     // places of this lane in a stage: K rows kperm(r32) (and 32 further), V as read_v8 takes it
     const int krow = kperm(r32), L = lane & 15;
@@ -284,10 +286,9 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       __syncthreads();
       if (t > 0) {
         copy_v(t, p0);
-        if (t + 1 < turns) copy_k(t + 1, p1);
+        if (t + 1 < turns) copy_k(t + 1, pages.page(p1));
       }
-      p0 = p1;
-      p1 = page_of(t + 2);
+      p0 = pages.page(p1);
       bf16x8 kf[2][2];
       auto read_k2 = [&](int s) {
 #pragma unroll
@@ -352,7 +353,11 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       // (formed here, between the products, not where they are used)
       asm volatile("" : "+v"(pn[2 * kh + (rr >> 3)][(rr & 7) / 2]), "+v"(ps));
     };
-    auto take = [&] {
+    auto take = [&](int t) {
+      // (the entry for the turn after the next: on its way while the copies are waited for, not while LDS reads are counted)
+      __builtin_amdgcn_sched_barrier(0);
+      p1 = entry_of(t + 2);
+      __builtin_amdgcn_sched_barrier(0);
       l += ps;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -364,12 +369,12 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     maxima();
 #pragma unroll
     for (int j = 0; j < 16; ++j) exps(j);
-    take();
+    take(0);
     for (int t = 1; t < turns; ++t) {
       first_product(t);
       const int rescale = maxima();
       second_product(exps);
-      take();
+      take(t);
       if (rescale) {   // (O has the page before by now, which the old maximum scaled)
 #pragma unroll
         for (int db = 0; db < 4; ++db) o[db] *= alpha;
