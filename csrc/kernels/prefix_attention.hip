@@ -86,8 +86,11 @@ __device__ __forceinline__ void load_q(const Args& A, int row, int head, int hh,
   const bf16* qp = A.q + (size_t)row * A.ldq + (size_t)head * HD + 8 * hh;
 #pragma unroll
   for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const bf16x8_u*>(qp + 16 * s);
+}
+// Waits for them (and with them for every copy so far): the first copies go out before, and from here on waits are counted
+__device__ __forceinline__ void have_q(bf16x8 (&qf)[8]) {
 #pragma unroll
-  for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(qf[s]));   // loaded before the copies are counted
+  for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(qf[s]));
 }
 
 // A lane's O (numbers 32 db + 8 g4 + 4 hh + 0 .. 3 of pair r32) as rows of 512 bytes in LDS, 16-byte piece p at p ^ r32
@@ -278,11 +281,8 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     };
     // S^T = K . Q^T of turn t's page, two halves of 32 keys; the copies of its V and of the next K go out first
     auto first_product = [&](int t) {
-      // K of this page and V of the one before have landed (at first: behind that K the first V and the next K); every wave is
-      // past the last page's K and the V before it
-      if (t > 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      else if (turns > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * CP) : "memory");
-      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CP) : "memory");
+      // K of this page and V of the one before have landed; every wave is past the last page's K and the V before it
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (t > 0) {
         copy_v(t, p0);
@@ -365,6 +365,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         pf[i >> 1][i & 1] = __builtin_bit_cast(bf16x8, u32x4{pn[i][0], pn[i][1], pn[i][2], pn[i][3]});
       }
     };
+    have_q(qf);
     first_product(0);
     maxima();
 #pragma unroll
@@ -484,6 +485,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     copy(A.kc, u0, page, false);
     copy(A.vc, u0, page, true);
     page = page_of(u0 + NW);
+    have_q(qf);
     for (int u = u0; u < u1; u += NW) {
       const bool more = u + NW < u1;
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");    // K (V's eight copies follow)
