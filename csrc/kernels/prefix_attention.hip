@@ -106,10 +106,12 @@ __device__ __forceinline__ f32x4 get_row(const float* so, int pair, int piece) {
   return *reinterpret_cast<const f32x4*>(so + pair * HD + ((piece ^ pair) << 2));
 }
 
-// where a pair's result of this part belongs
-__device__ __forceinline__ long part_at(const Args& A, const Work& W, int kvh, int pair) {
-  const int row = W.row0 + pair / A.G, before = A.even ? row * A.even : A.base[row];
-  return ((long)(before + W.slot + W.part) * A.Hkv + kvh) * A.G + pair % A.G;
+// Where a pair's numbers go: into out where its row has one part, else into the parts' outputs
+__device__ __forceinline__ long place_of(const Args& A, const Work& W, int kvh, int pair) {
+  const int row = W.row0 + pair / A.G, head = kvh * A.G + pair % A.G;
+  if (A.even == 1) return (long)row * A.ldo + head * HD;
+  const int before = A.even ? row * A.even : A.base[row];
+  return ((long)(before + W.slot + W.part) * A.Hkv * A.G + head) * HD;
 }
 
 // One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
@@ -152,8 +154,8 @@ __device__ void exact_pair(const Args& A, const int* btr, int r, int h, int lane
 }
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
-// Result of pair `pair` from its only part: lane r32 has numbers 4 r32 ..  A bit of `bad` says that it has to be done again.
-__device__ __forceinline__ bool put_result(const Args& A, const Work& W, int kvh, int pair, f32x4 sum, float den, int r32) {
+// A pair's result from its only part: lane r32 has numbers 4 r32 ..  True: it has to be done again.
+__device__ __forceinline__ bool put_result(const Args& A, long at, f32x4 sum, float den, int r32) {
   const float by = 1.f / den;
   bf16x4 y;
   bool bad = false;
@@ -163,8 +165,7 @@ __device__ __forceinline__ bool put_result(const Args& A, const Work& W, int kvh
     bad |= not_finite(x);
     y[i] = f2bf(x);
   }
-  bf16* op = A.out + (size_t)(W.row0 + pair / A.G) * A.ldo + (size_t)(kvh * A.G + pair % A.G) * HD + 4 * r32;
-  *reinterpret_cast<bf16x4_u*>(op) = y;
+  *reinterpret_cast<bf16x4_u*>(A.out + at + 4 * r32) = y;
   return bad;
 }
 __device__ void put_exact(const Args& A, const Work& W, int kvh, int pair, int lane) {
@@ -202,6 +203,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
   const Share S = share_of(W, W.of ? most_of(A, W, lane) : 0);
   const int pairs = W.n * A.G, mine = w * 32 + r32, pair = min(mine, pairs - 1), row = W.row0 + pair / A.G;
   const int lim = min(min(A.ctx_lens[row], A.max_ctx), S.end * PAGE), least = least_of(lim);
+  long to = S.first < S.end ? 0 : mine < pairs ? place_of(A, W, kvh, mine) : -1;
   f32x16 o[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -365,6 +367,8 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
         pf[i >> 1][i & 1] = __builtin_bit_cast(bf16x8, u32x4{pn[i][0], pn[i][1], pn[i][2], pn[i][3]});
       }
     };
+    to = mine < pairs ? place_of(A, W, kvh, mine) : -1;   // (while the copies are on their way)
+    asm volatile("" : "+v"(to));
     have_q(qf);
     first_product(0);
     maxima();
@@ -387,12 +391,10 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
-  const long to = mine >= pairs ? -1 : A.even == 1 ? 0 : part_at(A, W, kvh, mine);
   m = m == -INFINITY ? m : m * A.scale_log2;
-  if (!A.even == 1 && S.first >= S.end) {   // a part of no page has its maximum only
-    if (kg == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(m, l);
-    return;
-  }
+  const bool whole = A.even == 1;
+  if (!whole && (KG == 1 || S.first >= S.end) && kg == 0 && hh == 0 && to >= 0) A.part_ml[to / HD] = make_float2(m, l);
+  if (!whole && S.first >= S.end) return;   // a part of no page has its maximum only
   // the wavefront's rows to LDS and from there in whole rows, of both page groups: 32 / KG pairs for a wavefront
   float* so = reinterpret_cast<float*>(lds_all);
   put_rows(so + wave * (32 * HD), o, r32, hh);
@@ -408,24 +410,22 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
     const int p = kg * (32 / KG) + 2 * i + hh;
     const long at = __shfl(to, p, 64);
     f32x4 sum = get_row(so + w * (32 * HD), p, r32);
-    float M = __shfl(m, p, 64), den = __shfl(l, p, 64);
+    float den = KG == 1 && whole ? __shfl(l, p, 64) : 0.f;
     if constexpr (KG > 1) {
       const float2 a = sml[w * 32 + p], b = sml[(CW + w) * 32 + p];
-      M = fmaxf(a.x, b.x);
+      const float M = fmaxf(a.x, b.x);
       const float ea = a.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.x - M);
       const float eb = b.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(b.x - M);
       sum = sum * ea + get_row(so + (CW + w) * (32 * HD), p, r32) * eb;
       den = fmaf(ea, a.y, eb * b.y);
+      if (!whole && at >= 0 && r32 == 0) A.part_ml[at / HD] = make_float2(M, den);
     }
     if (at < 0) continue;
-    if (A.even == 1) {
-      bad |= (unsigned)put_result(A, W, kvh, w * 32 + p, sum, den, r32) << i;
-      continue;
-    }
-    *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = sum;
-    if (r32 == 0) A.part_ml[at] = make_float2(M, den);
+    if (whole) bad |= (unsigned)put_result(A, at, sum, den, r32) << i;
+    else *reinterpret_cast<f32x4*>(A.part_o + at + 4 * r32) = sum;
   }
-  if (__any(bad)) {
+  if (__builtin_expect(__any(bad), 0)) {
+#pragma unroll 1
     for (int i = 0; i < 32 / KG; ++i)
       if ((__ballot(bad >> (i / 2) & 1) >> (32 * (i & 1))) & 0xffffffffull)
         put_exact(A, W, kvh, w * 32 + kg * (32 / KG) + i, lane);
@@ -439,7 +439,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
 constexpr int KT = 32;
 
 template <int NW>
-__device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, int w, int lane) {
+__device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, bf16* lds_all, float2* sml, int w, int lane) {
   bf16* lds = lds_all + w * (2 * KT * HD);   // K and V; O at the end
   const int r32 = lane & 31, hh = lane >> 5;
   const Pages pages(A, W);
@@ -552,74 +552,64 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     }
   }
   l += __shfl_xor(l, 32, 64);
-  const long to = r32 >= pairs ? -1 : A.even == 1 ? 0 : part_at(A, W, kvh, r32);
-  if (!A.even == 1 && S.first >= S.end) {   // a part of no page has its maximum only
-    if (w == 0 && hh == 0 && to >= 0) A.part_ml[to] = make_float2(-INFINITY, 0.f);
+  const long to = r32 < pairs ? place_of(A, W, kvh, r32) : -1;
+  const bool whole = A.even == 1;
+  if (!whole && S.first >= S.end) {   // a part of no page has its maximum only
+    if (w == 0 && hh == 0 && to >= 0) A.part_ml[to / HD] = make_float2(-INFINITY, 0.f);
     return;
   }
-  // they meet: first their maxima and sums (where all wavefronts' copies have been), then O in their place
-  constexpr int EACH = ROWS * 32 / (NW * 64);   // 16-byte pieces of a thread
-  float2* sml = reinterpret_cast<float2*>(lds_all);
-  __syncthreads();
+  put_rows(reinterpret_cast<float*>(lds), o, r32, hh);   // (in this wavefront's own K and V)
   if (hh == 0) sml[w * ROWS + r32] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
-  __syncthreads();
-  float weight[EACH][NW], M[EACH], den[EACH];
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    float2 ml[NW];
-    M[i] = -INFINITY;
-    den[i] = 0.f;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      ml[x] = sml[x * ROWS + 2 * (NW * i + w) + hh];
-      M[i] = fmaxf(M[i], ml[x].x);
-    }
-#pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      weight[i][x] = ml[x].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[x].x - M[i]);
-      den[i] = fmaf(weight[i][x], ml[x].y, den[i]);
-    }
-  }
-  __syncthreads();
-  put_rows(reinterpret_cast<float*>(lds), o, r32, hh);
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(lds_all);
   unsigned bad = 0;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
+  for (int i = 0; i < ROWS * 32 / (NW * 64); ++i) {
     const int p = 2 * (NW * i + w) + hh;
     const long at = __shfl(to, p, 64);
-    if (at < 0) continue;
+    float2 ml[NW];
+    float M = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      ml[x] = sml[x * ROWS + p];
+      M = fmaxf(M, ml[x].x);
+    }
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < NW; ++x) sum += get_row(all + x * (KT * HD), p, r32) * weight[i][x];
-    if (A.even == 1) {
-      bad |= (unsigned)put_result(A, W, kvh, p, sum, den[i], r32) << i;
+    for (int x = 0; x < NW; ++x) {
+      const float e = ml[x].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[x].x - M);
+      den = fmaf(e, ml[x].y, den);
+      sum += get_row(all + x * (KT * HD), p, r32) * e;
+    }
+    if (at < 0) continue;
+    if (whole) {
+      bad |= (unsigned)put_result(A, at, sum, den, r32) << i;
       continue;
     }
-    *reinterpret_cast<f32x4*>(A.part_o + at * HD + 4 * r32) = sum;
-    if (r32 == 0) A.part_ml[at] = make_float2(M[i], den[i]);
+    *reinterpret_cast<f32x4*>(A.part_o + at + 4 * r32) = sum;
+    if (r32 == 0) A.part_ml[at / HD] = make_float2(M, den);
   }
-  if (__any(bad)) {
-    for (int i = 0; i < 2 * EACH; ++i)
+  if (__builtin_expect(__any(bad), 0)) {
+#pragma unroll 1
+    for (int i = 0; i < 2 * (ROWS * 32 / (NW * 64)); ++i)
       if ((__ballot(bad >> (i / 2) & 1) >> (32 * (i & 1))) & 0xffffffffull)
         put_exact(A, W, kvh, 2 * (NW * (i / 2) + w) + (i & 1), lane);
   }
 }
 
-template <int NW>
+template <int NW, bool TILES>   // TILES: some work has more than 32 pairs
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(
     Args A, const Work* __restrict__ works) {
   constexpr int KG = NW / 4;
   static_assert(NW * 2 * KT * HD == KG * 4 * PG, "both roles in the same LDS");
   __shared__ __attribute__((aligned(16))) bf16 lds[KG * 4 * PG];
-  __shared__ float2 sml[KG > 1 ? NW * 32 : 1];
+  __shared__ float2 sml[NW * 32];   // maxima and sums of every wavefront's pairs
   // heads first: with 8 kv heads an XCD has one of them, and its L2 that head's pages for all tiles
   const int b = blockIdx.x;
   const Work W = works[b / A.Hkv];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (W.n * A.G > ROWS) tile_role<KG>(A, W, b % A.Hkv, lds, sml, w, lane);
-  else few_role<NW>(A, W, b % A.Hkv, lds, w, lane);
+  if (TILES && W.n * A.G > ROWS) tile_role<KG>(A, W, b % A.Hkv, lds, sml, w, lane);
+  else few_role<NW>(A, W, b % A.Hkv, lds, sml, w, lane);
 }
 
 // The parts of a (row, head) pair: GROUPS half wavefronts, four numbers per lane, each with every GROUPS-th part.  A group has
@@ -711,15 +701,17 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* 
 // tables; part_o, part_ml: base[R] * Hq * (128 | 2) floats.  Every part of every row belongs to one work.
 P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int num_pages,
                                  const int* block_tables, int bt_stride, const int* ctx_lens, int max_ctx, const int* works,
-                                 int n_works, int waves, const int* base, const int* tables, int R, int parts, int even, int Hq, int Hkv,
+                                 int n_works, int waves, int tiles, const int* base, const int* tables, int R, int parts, int even, int Hq, int Hkv,
                                  int head_dim, float scale, void* out, int ldo, float* part_o, float* part_ml, hipStream_t stream) {
-  if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0) return (int)hipErrorInvalidValue;
+  if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0 || (waves != 4 && waves != 8))
+    return (int)hipErrorInvalidValue;
   const float sl2 = scale * 1.4426950408889634f;
   const int G = Hq / Hkv;
   const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, base, part_o,
                   (float2*)part_ml, (bf16*)out, ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G, even, sl2};
-  if (waves == 8) hipLaunchKernelGGL(prefix_attn_kernel<8>, dim3(n_works * Hkv), dim3(512), 0, stream, A, (const Work*)works);
-  else hipLaunchKernelGGL(prefix_attn_kernel<4>, dim3(n_works * Hkv), dim3(256), 0, stream, A, (const Work*)works);
+  const auto kernel = waves == 8 ? (tiles ? prefix_attn_kernel<8, true> : prefix_attn_kernel<8, false>)
+                                 : (tiles ? prefix_attn_kernel<4, true> : prefix_attn_kernel<4, false>);
+  hipLaunchKernelGGL(kernel, dim3(n_works * Hkv), dim3(waves * 64), 0, stream, A, (const Work*)works);
   if (int e = (int)hipGetLastError()) return e;
   if (even == 1) return 0;
   if (parts > 8 * R)

@@ -32,6 +32,7 @@ class PrefixPlan:
     max_ctx: int
     tables: int            # block tables it reads
     waves: int             # wavefronts of a workgroup, 4 or 8
+    tiles: bool            # some workgroup has more than FEW pairs
     even: int              # results of every row, where they are equally many (else 0)
     parts: int             # results of parts, over all rows
     works: torch.Tensor    # int32 [n, 8]
@@ -41,7 +42,7 @@ class PrefixPlan:
 
     def __post_init__(self):
         object.__setattr__(self, "launch", (
-            self.works.data_ptr(), self.works.shape[0], self.waves, self.base.data_ptr(), self.row_tables.data_ptr(), self.rows,
+            self.works.data_ptr(), self.works.shape[0], self.waves, self.tiles, self.base.data_ptr(), self.row_tables.data_ptr(), self.rows,
             self.parts, self.even, self.n_heads, self.n_kv, HEAD_DIM))
 
 
@@ -187,8 +188,9 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     flat = [x for w in works for x in w] + seqs + base
     flat = torch.tensor(flat, dtype=torch.int32).to(dev)
     n = 8 * len(works)
+    tiles = any(w[1] * (n_heads // n_kv) > FEW for w in works)
     even = count[0] if min(count) == max(count) else 0
-    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, waves, even, base[-1], flat[:n].view(-1, 8), flat[n + R:],
+    return PrefixPlan(R, n_heads, n_kv, max_ctx, max(seqs) + 1, waves, tiles, even, base[-1], flat[:n].view(-1, 8), flat[n + R:],
                       flat[n:n + R])
 
 
