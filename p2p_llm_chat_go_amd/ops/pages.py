@@ -91,6 +91,8 @@ def compact_pages_ref(k, v, block_tables, lens, keep, out_tables, cos_sin):
         new[b] = len(old)
         to = block_tables[b] if out_tables is None else out_tables[b]
         fp, tp = block_tables[b][old // PAGE].long(), to[n // PAGE].long()
+        pages = (fp >= 0) & (fp < k.shape[1]) & (tp >= 0) & (tp < k.shape[1])
+        old, n, fp, tp = old[pages], n[pages], fp[pages], tp[pages]
         x, y = k[:, fp, :, old % PAGE], v[:, fp, :, old % PAGE]       # token, layer, head, number
         if cos_sin is not None:
             a, c = cos_sin[old].double(), cos_sin[n].double()

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from p2p_llm_chat_go_amd import ops
+from p2p_llm_chat_go_amd.models.config import LLAMA31_8B, rope_table
 from p2p_llm_chat_go_amd.ops import prefix
 from tests import prefix_oracle as oracle
 
@@ -157,3 +158,17 @@ def test_compaction_that_is_refused(why, kw):
     a.update(kw)
     with pytest.raises(ValueError, match=why):
         ops.compact_pages(k, v, **a)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("turn", [False, True])
+def test_compaction_skips_entries_that_are_no_pages(apart, turn):
+    gen = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(2, 12, 2, PAGE, D, generator=gen).bfloat16() for _ in range(2))
+    table, to = torch.tensor([[1, 2, 10 ** 9], [4, -1, 5]], dtype=torch.int32), torch.tensor([[6, 12, 7], [-5, 8, 9]],
+                                                                                             dtype=torch.int32)
+    n, keep = torch.tensor([190, 150], dtype=torch.int32), torch.rand(2, 192, generator=gen) < 0.8
+    to, rot = to if apart else None, rope_table(LLAMA31_8B, max_pos=192) if turn else None
+    want_k, want_v, want_n, bound = oracle.compacted(k, v, table, n, keep, to, rot)
+    assert ops.compact_pages(k, v, table, n, keep, out_tables=to, cos_sin=rot).tolist() == want_n
+    assert torch.equal(v.double(), want_v) and bool(((k.double() - want_k).abs() <= bound).all())
