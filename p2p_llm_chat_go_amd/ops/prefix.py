@@ -20,6 +20,7 @@ from .attention import HEAD_DIM, PAGE, paged_attention_ref
 SCALE = 1.0 / math.sqrt(HEAD_DIM)
 SHARED_PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96)
 OWN_PARTS = (1, 2, 4, 8, 16, 32, 64)
+FAR = 2 ** 31          # strides are below
 FEW, MANY = 32, 128    # (row, head) pairs of a workgroup, in the kernel's two roles
 
 
@@ -42,8 +43,8 @@ class PrefixPlan:
 
     def __post_init__(self):
         object.__setattr__(self, "launch", (
-            self.works.data_ptr(), self.works.shape[0], self.waves, self.tiles, self.base.data_ptr(), self.row_tables.data_ptr(), self.rows,
-            self.parts, self.even, self.n_heads, self.n_kv, HEAD_DIM))
+            self.works.data_ptr(), self.works.shape[0], self.waves, self.tiles, self.base.data_ptr(), self.row_tables.data_ptr(),
+            self.rows, self.parts, self.even, self.n_heads, self.n_kv, HEAD_DIM))
 
 
 def _int(x, what: str) -> int:
@@ -160,7 +161,8 @@ def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None
     groups: (rows, pages) of every group, in the order of the rows: the next ``rows`` rows, whose block tables begin with the
     same ``pages`` pages (0: they share nothing).  seqs: every row's block-table row (rows of one sequence one after the
     other); None: row r has row r, as in a decode step.  max_ctx: the longest context that the plan is used for.  Context
-    lengths are not part of it: a decode step's plan serves its batch until a sequence joins or leaves."""
+    lengths are not part of it: a decode step's plan serves its batch until a sequence joins or leaves.  Its tensors are kept
+    until the calls that read them have ended, as any tensor that another stream than its own reads."""
     n_heads, n_kv, max_ctx = _int(n_heads, "n_heads"), _int(n_kv, "n_kv"), _int(max_ctx, "max_ctx")
     if n_kv < 1 or n_heads < n_kv or n_heads % n_kv or n_heads // n_kv > FEW:
         raise ValueError("prefix_plan: %d query heads on %d kv heads (1 to %d each)" % (n_heads, n_kv, FEW))
@@ -200,27 +202,38 @@ def prefix_workspace(plan: PrefixPlan) -> torch.Tensor:
     return torch.empty(plan.parts * plan.n_heads * (HEAD_DIM + 2), device=plan.works.device, dtype=torch.float32)
 
 
+def _overlap(q, out, R, width) -> bool:
+    """Whether the first R rows of q and out (bf16, ``width`` numbers each) have memory in common."""
+    sq, so, row = q.stride(0) * 2, out.stride(0) * 2, width * 2
+    ahead = out.data_ptr() - q.data_ptr()
+    if ahead >= (R - 1) * sq + row or -ahead >= (R - 1) * so + row:
+        return False
+    return sq != so or sq < row or ahead % sq < row or ahead % sq > sq - row
+
+
 def _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale):
     """Says which of prefix_attention's conditions does not hold."""
     R, n_heads, n_kv, width = plan.rows, plan.n_heads, plan.n_kv, plan.n_heads * HEAD_DIM
     def need(ok, why):
         if not ok:
             raise ValueError("prefix_attention: " + why)
-    need(q.dim() == 2 and q.dtype == torch.bfloat16 and q.shape[0] >= R and q.shape[1] == width and q.stride(1) == 1,
-         "q must be bf16 [%d or more, %d], rows contiguous" % (R, width))
+    need(q.dim() == 2 and q.dtype == torch.bfloat16 and q.shape[0] >= R and q.shape[1] == width and q.stride(1) == 1
+         and q.stride(0) < FAR, "q must be bf16 [%d or more, %d], rows contiguous" % (R, width))
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
         need(c.dim() == 4 and c.shape[1:] == (n_kv, PAGE, HEAD_DIM) and c.dtype == torch.bfloat16 and c.is_contiguous()
              and c.shape[0] > 0 and c.data_ptr() % 16 == 0,
              "%s must be bf16 [pages, %d, %d, %d], contiguous from a multiple of 16 bytes" % (name, n_kv, PAGE, HEAD_DIM))
     need(k_cache.shape == v_cache.shape, "k_cache and v_cache differ in shape")
     need(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
-         and block_tables.shape[0] >= plan.tables and block_tables.shape[1] * PAGE >= plan.max_ctx,
+         and block_tables.stride(0) < FAR and block_tables.shape[0] >= plan.tables and block_tables.shape[1] * PAGE >= plan.max_ctx,
          "block_tables must be int32 [%d or more, pages of %d tokens]" % (plan.tables, plan.max_ctx))
     need(ctx_lens.dim() == 1 and ctx_lens.dtype == torch.int32 and ctx_lens.shape[0] >= R and ctx_lens.stride(0) == 1,
          "ctx_lens must be int32 [%d or more]" % R)
     need(0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
-    need(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width and out.stride(1) == 1,
-         "out must be bf16 [%d or more, %d], rows contiguous" % (R, width))
+    need(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width and out.stride(1) == 1
+         and (out.stride(0) >= width or R == 1) and out.stride(0) < FAR,
+         "out must be bf16 [%d or more, %d], rows contiguous and apart" % (R, width))
+    need(not _overlap(q, out, R, width), "out overlaps q")
     need(all(t.device == q.device for t in (k_cache, v_cache, block_tables, ctx_lens, plan.works, out)),
          "tensors and plan must be on one device")
     need(workspace is None or (workspace.device == q.device and workspace.dtype == torch.float32 and workspace.is_contiguous()
@@ -235,8 +248,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """q: [R, n_heads * 128] bf16 -> out [R, n_heads * 128] bf16, as :func:`paged_attention` with the plan's tables.
 
     Row r attends the first ``min(ctx_lens[r], plan.max_ctx)`` tokens of its block table; a row that sees none is 0.  Rows
-    behind the plan's are not read or written.  A group's shared pages are read through its first row's table.  Block
-    tables hold pages of the cache; others read page 0 or the last one."""
+    behind the plan's are not read or written; out is other memory than q.  A group's shared pages are read through its
+    first row's table.  Block tables hold pages of the cache; others read page 0 or the last one."""
     R, n_heads, n_kv = plan.rows, plan.n_heads, plan.n_kv
     width = n_heads * HEAD_DIM
     if scale is None:
@@ -261,7 +274,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
               and k_cache.is_contiguous() and v_cache.is_contiguous() and 0 < scale < math.inf
               and dev == out.get_device() == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
               == ctx_lens.get_device() == works.get_device())
-        kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+        kp, vp, qp, op, sq, so = k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0)
+        if qp + 2 * (R * sq + width) > op and op + 2 * (R * so + width) > qp:
+            ok = ok and not _overlap(q, out, R, width)
+        ok = ok and (so >= width or R == 1) and sq < FAR > so and block_tables.stride(0) < FAR
         if ok and dev >= 0:
             wp = workspace.data_ptr()
             ok = ((kp | vp | wp) % 16 == 0 and workspace.get_device() == dev and workspace.dtype == torch.float32
@@ -282,7 +298,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         with torch.cuda.device(dev):
             return prefix_attention(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale)
     _lib.check(_lib.lib().p2p_prefix_attention(
-        q.data_ptr(), q.stride(0), kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx,
-        *plan.launch, scale, out.data_ptr(), out.stride(0), wp, wp + plan.parts * width * 4,
+        qp, sq, kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx,
+        *plan.launch, scale, op, so, wp, wp + plan.parts * width * 4,
         torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
     return out

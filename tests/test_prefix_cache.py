@@ -91,11 +91,32 @@ def _given(**kw):
     ("ctx_lens", dict(ctx_lens=torch.zeros(2, dtype=torch.int32))), ("ctx_lens", dict(ctx_lens=torch.zeros(3))),
     ("scale", dict(scale=0.0)), ("scale", dict(scale=-1.0)), ("scale", dict(scale=float("nan"))),
     ("out must", dict(out=torch.zeros(3, 4 * D))), ("out must", dict(out=torch.zeros(2, 4 * D, dtype=BF))),
+    ("out must", dict(out=torch.zeros(4 * D, dtype=BF).expand(3, -1))),
+    ("q must", dict(q=torch.zeros(1, 1, dtype=BF, device="meta").as_strided((3, 4 * D), (2 ** 31, 1)))),
     ("one device", dict(ctx_lens=torch.zeros(3, dtype=torch.int32, device="meta"))),
 ])
 def test_attention_that_is_refused(why, kw):
     with pytest.raises(ValueError, match=why):
         ops.prefix_attention(**_given(**kw))
+
+
+@pytest.mark.parametrize("qs,outs,ok", [
+    ((0, 4 * D), (0, 4 * D), False), ((0, 4 * D), (4 * D, 4 * D), False), ((0, 4 * D), (12 * D, 4 * D), True),
+    ((12 * D, 4 * D), (0, 4 * D), True), ((0, 8 * D), (4 * D, 8 * D), True), ((4 * D, 8 * D), (0, 8 * D), True),
+    ((0, 8 * D), (4 * D - 1, 8 * D), False), ((4 * D - 1, 8 * D), (0, 8 * D), False), ((0, 8 * D), (5 * D, 8 * D), False),
+    ((0, 4 * D), (8 * D, 6 * D), False), ((0, 4 * D), (12 * D, 6 * D), True),
+    ((0, 0), (0, 4 * D), False), ((0, 0), (4 * D, 4 * D), True), ((5 * D, 0), (0, 4 * D), False),
+])
+def test_out_is_other_memory_than_q(qs, outs, ok):
+    """(start, stride) of both in one buffer: rows that lie between one another are fine."""
+    buffer = torch.randn(60 * D).to(BF)
+    a = _given(q=buffer.as_strided((3, 4 * D), (qs[1], 1), qs[0]), out=buffer.as_strided((3, 4 * D), (outs[1], 1), outs[0]))
+    if ok:
+        want = ops.prefix_attention(**dict(a, out=None))
+        assert torch.equal(ops.prefix_attention(**a), want)
+    else:
+        with pytest.raises(ValueError, match="out overlaps q"):
+            ops.prefix_attention(**a)
 
 
 def test_attention_on_the_cpu():
