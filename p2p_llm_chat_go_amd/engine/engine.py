@@ -53,7 +53,7 @@ def common_prefix(prompts: list) -> int:
     first = prompts[0]
     for p in prompts[1:]:
         if p[:n] != first[:n]:
-            n = next(i for i in range(n) if p[i] != first[i])
+            n = next((i for i in range(n) if p[i] != first[i]), n)
     return max(n, 0)
 
 

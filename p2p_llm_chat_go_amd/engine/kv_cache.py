@@ -44,11 +44,19 @@ class PageAllocator:
         """Whether more than one sequence owns the page."""
         return page in self._more
 
-    def share(self, pages):
-        """One more owner for each of the pages (which are in use); each owner frees them once."""
+    def owners(self, page: int) -> int:
+        """How many sequences own a page that is in use."""
+        return 1 + self._more.get(page, 0)
+
+    def check(self, pages):
+        """Raises where one of them is no page that a sequence can own."""
         for p in pages:
             if p <= 0 or p >= self.num_pages:
                 raise ValueError("bad page %d" % p)
+
+    def share(self, pages):
+        """One more owner for each of the pages (which are in use); each owner frees them once."""
+        self.check(pages)
         for p in pages:
             self._more[p] = self._more.get(p, 0) + 1
 
@@ -59,9 +67,7 @@ class PageAllocator:
         return out
 
     def free(self, pages):
-        for p in pages:
-            if p <= 0 or p >= self.num_pages:
-                raise ValueError("bad page %d" % p)
+        self.check(pages)
         for p in pages:
             more = self._more.get(p)
             if more is None:
@@ -118,6 +124,7 @@ class KVCache:
         full, need = tokens // PAGE, pages_for(tokens)
         if any(n < need for n in sizes):
             raise ValueError("fork: %d tokens take %d pages, asked for %d" % (tokens, need, min(sizes)))
+        self.allocator.check(pages[:need])
         fresh = self.allocator.alloc(sum(n - full for n in sizes))
         out, at = [], 0
         for n in sizes:
@@ -136,16 +143,18 @@ class KVCache:
         ones; pages that nobody owns any more are free.  cos_sin (``LlamaModel.rope``): keys are turned to their new
         positions, and the sequence goes on at its new length; None: it goes on counting from where it was, and only the
         cache's places change."""
-        dev = self.k.device
         keep = torch.as_tensor(keep, dtype=torch.bool)
         if keep.dim() != 2 or keep.shape[0] != len(pages) or len(lens) != len(pages):
             raise ValueError("compact: %d sequences, %d lengths, keep %s" % (len(pages), len(lens), list(keep.shape)))
         for p, n in zip(pages, lens):
             if not 0 <= n <= min(len(p) * PAGE, keep.shape[1]):
                 raise ValueError("compact: a length of %d with %d pages and %d places in keep" % (n, len(p), keep.shape[1]))
+        if room < 0:
+            raise ValueError("compact: room for %d tokens" % room)
         given = collections.Counter(p for q in pages for p in q)
-        if any(n > 1 and not self.allocator.shared(p) for p, n in given.items()):
-            raise ValueError("compact: a page is given twice")
+        self.allocator.check(given)
+        if any(n > self.allocator.owners(p) for p, n in given.items()):
+            raise ValueError("compact: a page is given twice, or by more sequences than own it")
         if not pages:
             return [], []
         lens_t = torch.tensor(lens, dtype=torch.int32)
@@ -153,7 +162,11 @@ class KVCache:
         left = (host & (torch.arange(host.shape[1]) < lens_t[:, None])).sum(1).tolist()
         size = [pages_for(n + room) for n in left]
         apart = [any(self.allocator.shared(p) for p in q) for q in pages]
-        # new pages first: nothing has changed when there are none
+        # what the moves would refuse, then the new pages: nothing has changed where either fails
+        dev = self.k.device
+        none = torch.zeros(0, max(map(len, pages)), dtype=torch.int32, device=dev)
+        keep = keep.to(dev)
+        compact_pages(self.k, self.v, none, none.new_zeros(0), keep[:0], cos_sin=cos_sin)
         fresh = self.allocator.alloc(sum(n if a else max(0, n - len(q)) for n, a, q in zip(size, apart, pages)))
         out, gone = [], []
         for n, a, q in zip(size, apart, pages):
@@ -161,7 +174,6 @@ class KVCache:
             mine, fresh = fresh[:take], fresh[take:]
             out.append(mine if a else q[:n] + mine)
             gone += q if a else q[n:]
-        keep = keep.to(dev)
         for way in (False, True):
             at = [i for i, a in enumerate(apart) if a == way and lens[i]]
             if not at:

@@ -113,7 +113,7 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
 
     block_tables: int32 [B, pages]; lens: int32 [B], the sequences' tokens (at most the table's and keep's); keep: bool
     [B, tokens].  out_tables: int32 like block_tables, the pages that the tokens go to, none of them in block_tables; None: in
-    place.  In place no page may belong to two of the sequences.  Rows of pages behind the new lengths stay as they were.
+    place.  In place no page is in the tables twice.  Rows of pages behind the new lengths stay as they were.
     cos_sin: float32 [positions, 64, 2] (``models.config.rope_table``): keys that were rotated for position p are turned on to
     position n (bf16 caches); None: they stay as they are, as for sequences that go on counting positions.  Entries of the
     tables that are no pages are skipped."""
@@ -129,6 +129,7 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
     need(keep.dim() == 2 and keep.dtype == torch.bool and keep.shape[0] == B and (keep.stride(1) == 1 or keep.shape[1] < 2),
          "keep must be bool [%d, tokens]" % B)
     need(B <= 65535, "more than 65535 sequences")
+    need(all(t is None or t.stride(0) < 2 ** 31 for t in (block_tables, out_tables)), "tables with rows too far apart")
     if out_tables is not None:
         need(out_tables.dtype == torch.int32 and out_tables.shape == block_tables.shape
              and (out_tables.stride(1) == 1 or W < 2), "out_tables must be like block_tables")

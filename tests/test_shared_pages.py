@@ -79,6 +79,9 @@ def test_forks_that_are_refused():
             kv.fork(mine, tokens, sizes)
     with pytest.raises(MemoryError):
         kv.fork(mine, 64, [3, 3])
+    for bad in ([0, mine[1]], [mine[0], 6], [mine[0], -1]):
+        with pytest.raises(ValueError, match="bad page"):
+            kv.fork(bad, 70, [2])
     assert kv.allocator.free_pages == 3 and not kv.allocator.shared(mine[0])
 
 
@@ -128,10 +131,20 @@ def test_compactions_that_are_refused():
             kv.compact(*args)
     with pytest.raises(MemoryError):
         kv.compact([a], [100], keep, room=1000)
+    b, = kv.fork(a, 128, [2])
+    for args, kw, why in ((([a, b, a], [9] * 3, keep.repeat(3, 1)), {}, "more sequences than own it"),
+                          (([a], [100], keep), dict(room=-1), "room for -1"), (([[a[0], 8]], [9], keep), {}, "bad page 8"),
+                          (([[0]], [9], keep), {}, "bad page 0"), (([a], [9], keep), dict(cos_sin=torch.zeros(9, 64, 2)), "cos_sin")):
+        with pytest.raises(ValueError, match=why):
+            kv.compact(*args, **kw)
     assert kv.compact([], [], keep[:0]) == ([], [])
+    kv.allocator.free(a)
+    kv.allocator.free(b)
+    assert kv.allocator.free_pages == 7
 
 
 def test_common_prefixes():
+    assert common_prefix([[1, 2, 3], (1, 2, 3, 4)]) == 2
     assert common_prefix([[1, 2, 3], [1, 2, 4, 5]]) == 2 and common_prefix([[1, 2, 3], [1, 2, 3]]) == 2
     assert common_prefix([[1], [1, 2]]) == 0 and common_prefix([[5, 6], [1, 6]]) == 0
 
