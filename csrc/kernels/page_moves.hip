@@ -241,18 +241,20 @@ __global__ __launch_bounds__(1024) void compact_inside_kernel(Cache k, Cache v, 
 template <int TPT, bool TURN>
 int compact(Cache k, Cache v, const Sequences& s, int n, int heads, int layers, const float* cos_sin, hipStream_t st) {
   if (!s.to) {
-    const int groups = heads * layers * n;
-    constexpr int MANY = TURN ? 2 : 1;
-    if (MANY > 1 && heads % MANY == 0 && groups / MANY >= 192)
-      hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN, MANY>), dim3(heads / MANY * layers, n), dim3(1024), 0, st, k, v, s, heads,
-                         cos_sin);
+    // Two heads in flight per workgroup, once that leaves 192 workgroups: six sequences of 8150 places in 8 layers turned
+    // 613 -> 450 us, as they are 416 -> 352, six of 1000 66 -> 48 and 45 -> 39; three of 1000 would lose, 36 -> 41 and 25 -> 30.
+    if (heads % 2 == 0 && heads * layers * n >= 384)
+      hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN, 2>), dim3(heads / 2 * layers, n), dim3(1024), 0, st, k, v, s, heads, cos_sin);
     else
       hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN, 1>), dim3(heads * layers, n), dim3(1024), 0, st, k, v, s, heads, cos_sin);
     return (int)hipGetLastError();
   }
   constexpr int TOK = 256 / TPT;
-  const int chunks = max(1, (min(s.places, s.width * PAGE) + TOK - 1) / TOK);
-  const int shares = max(1, min(heads * layers / 8, 8192 / max(1, chunks * n)));
+  const int chunks = max(1, (min(s.places, s.width * PAGE) + TOK - 1) / TOK), all = heads * layers;
+  // Eight (layer, head) pairs for a workgroup, which counts kept places and forms angles once for them: six sequences of 8150
+  // places in 8 layers turned 331 us, with one pair each 448, with all 64 349 (as they are 328, 338, 347).  Fewer where
+  // there would not be 256 workgroups: one layer of 1000 places 7.6 -> 6.3.
+  const int shares = max(max(1, all / 8), min(all, 256 / max(1, chunks * n)));
   hipLaunchKernelGGL((compact_apart_kernel<TPT, TURN>), dim3(chunks, n, shares), dim3(256), 0, st, k, v, s, heads, layers, cos_sin);
   return (int)hipGetLastError();
 }
