@@ -714,7 +714,10 @@ P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, co
   hipLaunchKernelGGL(kernel, dim3(n_works * Hkv), dim3(waves * 64), 0, stream, A, (const Work*)works);
   if (int e = (int)hipGetLastError()) return e;
   if (even == 1) return 0;
-  if (parts > 8 * R)
+  // A workgroup for each pair where pairs are few, a half wavefront where they fill the chip.  64 pairs of 8 parts 12.8 -> 11.0 us
+  // with the parts' own time, of 24 15.9 -> 9.2; 608 of 8 22.2 -> 20.6, 2048 of 10 23.6 -> 22.6 (of 2 80.0 -> 81.3); 4096 of 10
+  // 29.1 and 29.5, 8192 of 10 54.5 and 57.3.
+  if (parts > 3 * R && R * Hq <= 2048)
     hipLaunchKernelGGL(prefix_combine_kernel<8>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R);
   else
     hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 7) / 8), dim3(256), 0, stream, A, tables, R);

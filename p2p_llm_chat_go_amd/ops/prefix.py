@@ -104,43 +104,45 @@ class _Shape:
 
     def micros(self, waves: int, share: bool, shared_parts: int, own_parts: int) -> float:
         """About how long a call takes: constants fitted to timings of 78 batches, of 2 to 768 rows behind 128 to 32768 tokens, cut
-        in all ways.  A launch and its first loads 3.2 us (of 8 wavefronts 4.6); a page of a tile of 128 pairs 1.2 us where CUs
-        have one workgroup, 1.4 where they have two, two pages of 8 wavefronts 2.1; 32 keys of a wavefront 1.05 (1.2); what memory
-        and L2 add, as if they were three sides of a box, at 8.5 and 24 TB/s; a second launch 4.5, 0.6 per MB of the parts'
-        results, and 0.08 for every part of a row; rows alone in parts a tenth more than that.  The cut that it puts first takes
-        3.0 % longer than the fastest one on average (with 4 wavefronts only: 5.7 %)."""
+        in all ways.  A launch and its first loads 4.1 us (of 8 wavefronts 5.2); a page of a tile of 128 pairs 1.25 us where CUs
+        have one workgroup, 1.4 where they have two, two pages of 8 wavefronts 2.25; 32 keys of a wavefront 0.65 (0.8); what memory
+        and L2 add, as if they were three sides of a box, at 17.5 and 25 TB/s (the caches held much of it); a second launch 2.1,
+        0.84 per MB of the parts' results; rows alone in parts a twentieth more.  The cut that it puts first takes 2.8 % longer
+        than the fastest one on average."""
         many = few = many_pages = few_units = parts = read = loaded = 0
         for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
-            own = (self.pages - p + 1) // 2       # (contexts end somewhere up to the plan's longest)
+            # contexts end somewhere up to the plan's longest: half of the pages on average, some tokens more in the longest
+            own = (self.pages - p + 1) // 2
+            longest = min(self.pages - p, own + 4)
             read += p + runs * own
             if share and p:
-                todo = ((tiles, tiles_many, p, min(shared_parts, -(-p // 2))),
-                        (runs, runs_many, own, min(own_parts, -(-(self.pages - p) // 2))))
+                todo = ((tiles, tiles_many, p, p, min(shared_parts, -(-p // 2))),
+                        (runs, runs_many, own, longest, min(own_parts, -(-longest // 2))))
             else:
-                todo = ((runs, runs_many, p + own, min(own_parts, -(-self.pages // 2))),)
-            for n, is_many, pages, C in todo:
+                todo = ((runs, runs_many, p + own, self.pages, min(own_parts, -(-self.pages // 2))),)
+            for n, is_many, pages, most_pages, C in todo:
                 if not C:
                     continue
                 parts += rows * C
                 loaded += n * pages
                 if is_many:
                     many += n * C * self.n_kv
-                    many_pages = max(many_pages, -(-pages // C))
+                    many_pages = max(many_pages, -(-most_pages // C))
                 else:
                     few += n * C * self.n_kv
-                    few_units = max(few_units, -(-pages // (2 * C)))
+                    few_units = max(few_units, -(-most_pages // (2 * C)))
         eight, most = waves == 8, 2048 // waves        # (workgroups at once)
         if eight:
             many_pages, few_units = -(-many_pages // 2), -(-few_units // 2)
-        t_many = many_pages * (2.1 if eight else 1.2 if many <= 256 else 1.4) * max(1.0, many / most)
-        t_few = few_units * (1.2 if eight else 1.05) * max(1.0, few / most)
+        t_many = many_pages * (2.25 if eight else 1.25 if many <= 256 else 1.4) * -(-many // most)
+        t_few = few_units * (0.8 if eight else 0.65) * -(-few // most)
         t = max(t_many, t_few) if many + few <= most else t_many + t_few
         page = self.n_kv * 32768e-6                    # MB
-        t = (4.6 if eight else 3.2) + math.hypot(t, read * page / 8.5, loaded * page / 24)
+        t = (5.2 if eight else 4.1) + math.hypot(t, read * page / 17.5, loaded * page / 25)
         if parts > self.R:
-            t += 4.5 + 0.6e-6 * parts * self.n_heads * 512 + 0.08 * parts / self.R
+            t += 2.1 + 0.84e-6 * parts * self.n_heads * 512
             if not share:
-                t *= 1.1
+                t *= 1.05
         return t
 
     def choose(self):

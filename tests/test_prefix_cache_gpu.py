@@ -94,6 +94,16 @@ def test_prefix_attention_in_many_parts(groups, own, monkeypatch):
     _check(_run(q, k, v, table, ctx, plan), want, bound)
 
 
+def test_prefix_attention_of_many_rows_in_many_parts(monkeypatch):
+    """More than 2048 pairs of a row and a head, some of one part, others of 21."""
+    monkeypatch.setattr(prefix._Shape, "choose", lambda self: (4, True, 20, 1))
+    q, k, v, table, seqs, ctx, rows, most = _batch([(250, 40), (11, 0)], 8, 1, 3, 1)
+    plan = ops.prefix_plan(rows, 8, 1, most, DEV)
+    assert plan.even == 0 and plan.parts == 250 * 21 + 11
+    want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 1, 1 / math.sqrt(D), most)
+    _check(_run(q, k, v, table, ctx, plan), want, bound)
+
+
 @pytest.mark.parametrize("Hq,Hkv", [(8, 2), (4, 4), (8, 1), (3, 1)])
 @pytest.mark.parametrize("groups,own,tokens", [([(3, 2)], 44, 44), ([(2, 4), (3, 1)], 100, 17), ([(1, 5)], 200, 130),
                                                ([(9, 1)], 64, 2)])
