@@ -7,6 +7,10 @@
 // o = sum_c exp(m_c - M) o_c / sum_c exp(m_c - M) l_c with M = max m_c.  So a row's keys may be cut anywhere and each piece
 // be done together with other rows that see the same keys.  The host cuts the batch into works (`Work`): query rows of one
 // group (or of one sequence) against a range of pages, in `of` parts; the parts' results (fp32) meet in a second launch.
+//
+// What it takes, calls one after the other: 2 rows behind 256 tokens 7 us (the host 10), 19 behind 2048 13 and 41 on one kv head
+// 15, of which the second launch is 3: chains of loads of some 0.7 us each (work, page numbers, keys, values) and the launches.
+// 704 prompt rows behind 1536 tokens 34 us, 64 rows of 64 heads behind 32768 107 us: the products, see the tiles.
 #include "common.h"
 #include "lds_pipe.h"
 
@@ -191,8 +195,16 @@ __device__ __forceinline__ bf16x8 read_v8(const bf16* p) {
 // Four wavefronts have 32 pairs each and share the pages; with KG = 2 four more have the same pairs and every other page (two
 // pages of a workgroup on its way, one result of them: half the results of two workgroups).  K and V of a page come by LDS DMA,
 // two stages each, and a page's exponentials run between the products of the page before with V, as in flash_prefill2_kernel
-// (whose layouts these are).  P is rounded to bf16 for the product (relative 2^-9: what a value's weight is off by); scores,
-// maxima, sums and O are fp32.
+// (whose layouts these are).  P is rounded to bf16 for the product (relative 2^-8 at most: what a value's weight is off by);
+// scores, maxima, sums and O are fp32.
+//
+// A wavefront reads a page's K and V from LDS, 32 KB, for 32 matrix instructions of 32 cycles: two workgroups on a CU have 2050
+// cycles of either for a page each, and take 2980 (one alone 2480 for 1024 of each).  The rest is the maxima, on which the
+// exponentials wait, and the wait for copies at a page's start.  64 rows of 64 heads behind 32768 tokens: 70 GFLOP in 100 us.
+// Three stages of K, a barrier of its own for V, copies spread between the products, LDS reads three pairs ahead and both
+// products interleaved (which spills) gave nothing.
+// 128 pairs, since a wavefront's registers hold 32 (O 64, Q 64, S and P 64) and four are a CU's quarters: with 32 pairs for a
+// workgroup 241 us, 129 then with 128.
 template <int KG>
 __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh, bf16* lds_all, float2* sml, int wave, int lane) {
   constexpr int CW = 4, CP = 16 / CW;                       // wavefronts that copy a page together, copies of each
@@ -435,7 +447,8 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
 // ---- up to 32 pairs ----
 // NW wavefronts, each with its own 32 keys at a time against the same pairs.  K and V come by LDS DMA into the wavefront's
 // own LDS, the next K while this one's weights are formed, the next V behind the second product; no barrier until they meet at
-// the end.
+// the end.  For up to 32 pairs, where of a tile's four wavefronts three had nothing to do: so they take different keys instead,
+// and a CU has four streams of loads, which is what few rows are bound by.  2 rows behind 1024 tokens, 6 MB, 8.2 us.
 constexpr int KT = 32;
 
 template <int NW>
@@ -614,6 +627,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
 // The parts of a (row, head) pair: GROUPS half wavefronts, four numbers per lane, each with every GROUPS-th part.  A group has
 // the statistics and outputs of eight parts in flight together, what they weigh is known when they have come; groups meet in LDS.
+// Bound by memory where there is much (4096 pairs of 17 parts, 36 MB, 9.5 us = 3.8 TB/s), else by its launch: 608 pairs 3 us.
 template <int GROUPS>
 __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* __restrict__ tables, int R) {
   const int Hq = A.Hkv * A.G, lane = threadIdx.x & 63, r32 = lane & 31, g = GROUPS == 1 ? 0 : threadIdx.x >> 5;
@@ -697,12 +711,14 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* 
 
 }  // namespace
 
-// works: int32 [n_works, 8] (Work); base: int32 [R + 1], the parts of the rows before (even: every row has so many, or 0); tables: int32 [R], the rows' block
-// tables; part_o, part_ml: base[R] * Hq * (128 | 2) floats.  Every part of every row belongs to one work.
+// works: int32 [n_works, 8] (Work); tiles: some work has more than 32 pairs; base: int32 [R + 1], the parts of the rows before
+// (even: every row has so many, or 0); tables: int32 [R], the rows' block tables; part_o, part_ml: base[R] * Hq * (128 | 2)
+// floats.  Every part of every row belongs to one work.
 P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int num_pages,
                                  const int* block_tables, int bt_stride, const int* ctx_lens, int max_ctx, const int* works,
-                                 int n_works, int waves, int tiles, const int* base, const int* tables, int R, int parts, int even, int Hq, int Hkv,
-                                 int head_dim, float scale, void* out, int ldo, float* part_o, float* part_ml, hipStream_t stream) {
+                                 int n_works, int waves, int tiles, const int* base, const int* tables, int R, int parts,
+                                 int even, int Hq, int Hkv, int head_dim, float scale, void* out, int ldo, float* part_o,
+                                 float* part_ml, hipStream_t stream) {
   if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0 || (waves != 4 && waves != 8))
     return (int)hipErrorInvalidValue;
   const float sl2 = scale * 1.4426950408889634f;

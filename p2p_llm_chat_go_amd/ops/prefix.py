@@ -107,7 +107,7 @@ class _Shape:
         in all ways.  A launch and its first loads 4.1 us (of 8 wavefronts 5.2); a page of a tile of 128 pairs 1.25 us where CUs
         have one workgroup, 1.4 where they have two, two pages of 8 wavefronts 2.25; 32 keys of a wavefront 0.65 (0.8); what memory
         and L2 add, as if they were three sides of a box, at 17.5 and 25 TB/s (the caches held much of it); a second launch 2.1,
-        0.84 per MB of the parts' results; rows alone in parts a twentieth more.  The cut that it puts first takes 2.8 % longer
+        0.84 per MB of the parts' results; rows alone in parts a twentieth more.  The cut that it puts first takes 2.4 % longer
         than the fastest one on average."""
         many = few = many_pages = few_units = parts = read = loaded = 0
         for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
