@@ -711,31 +711,38 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* 
 
 }  // namespace
 
-// works: int32 [n_works, 8] (Work); tiles: some work has more than 32 pairs; base: int32 [R + 1], the parts of the rows before
-// (even: every row has so many, or 0); tables: int32 [R], the rows' block tables; part_o, part_ml: base[R] * Hq * (128 | 2)
-// floats.  Every part of every row belongs to one work.
-P2P_API int p2p_prefix_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int num_pages,
-                                 const int* block_tables, int bt_stride, const int* ctx_lens, int max_ctx, const int* works,
-                                 int n_works, int waves, int tiles, const int* base, const int* tables, int R, int parts,
-                                 int even, int Hq, int Hkv, int head_dim, float scale, void* out, int ldo, float* part_o,
-                                 float* part_ml, hipStream_t stream) {
-  if (head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || n_works <= 0 || (waves != 4 && waves != 8))
+// What a plan hands to its calls (host memory).
+struct PrefixPlan {
+  const int *works;       // int32 [n_works, 8] (Work); every part of every row belongs to one
+  const int *base;        // int32 [R + 1], the parts of the rows before
+  const int *tables;      // int32 [R], the rows' block tables
+  int n_works, waves, tiles, R, parts, even, Hq, Hkv, head_dim, max_ctx;   // tiles: some work has more than 32 pairs; even:
+};                                                                         // the parts of every row, or 0
+
+// workspace: parts * Hq * (128 + 2) floats, outputs and then maxima and sums.
+P2P_API int p2p_prefix_attention(const PrefixPlan* plan, const void* q, int ldq, const void* k_cache, const void* v_cache,
+                                 int num_pages, const int* block_tables, int bt_stride, const int* ctx_lens, float scale, void* out,
+                                 int ldo, float* workspace, hipStream_t stream) {
+  const PrefixPlan& P = *plan;
+  const int Hq = P.Hq, Hkv = P.Hkv, R = P.R, even = P.even;
+  if (P.head_dim != HD || Hkv <= 0 || Hq % Hkv || Hq / Hkv > ROWS || R <= 0 || P.n_works <= 0 || (P.waves != 4 && P.waves != 8))
     return (int)hipErrorInvalidValue;
   const float sl2 = scale * 1.4426950408889634f;
   const int G = Hq / Hkv;
-  const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, base, part_o,
-                  (float2*)part_ml, (bf16*)out, ldq, ldo, num_pages, bt_stride, max_ctx, Hkv, G, even, sl2};
-  const auto kernel = waves == 8 ? (tiles ? prefix_attn_kernel<8, true> : prefix_attn_kernel<8, false>)
-                                 : (tiles ? prefix_attn_kernel<4, true> : prefix_attn_kernel<4, false>);
-  hipLaunchKernelGGL(kernel, dim3(n_works * Hkv), dim3(waves * 64), 0, stream, A, (const Work*)works);
+  const Args A = {(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_tables, ctx_lens, P.base, workspace,
+                  (float2*)(workspace + (size_t)P.parts * Hq * HD), (bf16*)out, ldq, ldo, num_pages, bt_stride, P.max_ctx, Hkv, G,
+                  even, sl2};
+  const auto kernel = P.waves == 8 ? (P.tiles ? prefix_attn_kernel<8, true> : prefix_attn_kernel<8, false>)
+                                   : (P.tiles ? prefix_attn_kernel<4, true> : prefix_attn_kernel<4, false>);
+  hipLaunchKernelGGL(kernel, dim3(P.n_works * Hkv), dim3(P.waves * 64), 0, stream, A, (const Work*)P.works);
   if (int e = (int)hipGetLastError()) return e;
   if (even == 1) return 0;
   // A workgroup for each pair where pairs are few, a half wavefront where they fill the chip.  64 pairs of 8 parts 12.8 -> 11.0 us
   // with the parts' own time, of 24 15.9 -> 9.2; 608 of 8 22.2 -> 20.6, 2048 of 10 23.6 -> 22.6 (of 2 80.0 -> 81.3); 4096 of 10
   // 29.1 and 29.5, 8192 of 10 54.5 and 57.3.
-  if (parts > 3 * R && R * Hq <= 2048)
-    hipLaunchKernelGGL(prefix_combine_kernel<8>, dim3(R * Hq), dim3(256), 0, stream, A, tables, R);
+  if (P.parts > 3 * R && R * Hq <= 2048)
+    hipLaunchKernelGGL(prefix_combine_kernel<8>, dim3(R * Hq), dim3(256), 0, stream, A, P.tables, R);
   else
-    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 7) / 8), dim3(256), 0, stream, A, tables, R);
+    hipLaunchKernelGGL(prefix_combine_kernel<1>, dim3((R * Hq + 7) / 8), dim3(256), 0, stream, A, P.tables, R);
   P2P_CHECK_LAUNCH();
 }

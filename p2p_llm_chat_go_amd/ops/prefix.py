@@ -8,6 +8,7 @@ and a context length.
 """
 from __future__ import annotations
 
+import ctypes
 import dataclasses
 import math
 import operator
@@ -22,6 +23,13 @@ SHARED_PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96)
 OWN_PARTS = (1, 2, 4, 8, 16, 32, 64)
 FAR = 2 ** 31          # strides are below
 FEW, MANY = 32, 128    # (row, head) pairs of a workgroup, in the kernel's two roles
+
+
+class _Launch(ctypes.Structure):
+    """What a plan hands to its calls (PrefixPlan in the kernels' source)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("works", "base", "row_tables")]
+                + [(n, ctypes.c_int) for n in ("n_works", "waves", "tiles", "rows", "parts", "even", "n_heads", "n_kv", "head_dim",
+                                               "max_ctx")])
 
 
 @dataclasses.dataclass(frozen=True)
@@ -39,12 +47,14 @@ class PrefixPlan:
     works: torch.Tensor    # int32 [n, 8]
     base: torch.Tensor     # int32 [rows + 1]: parts of the rows before
     row_tables: torch.Tensor   # int32 [rows]
-    launch: tuple = dataclasses.field(init=False, repr=False, compare=False)   # what every call hands on of it
+    launch: _Launch = dataclasses.field(init=False, repr=False, compare=False)
+    at: int = dataclasses.field(init=False, repr=False, compare=False)     # its address
 
     def __post_init__(self):
-        object.__setattr__(self, "launch", (
-            self.works.data_ptr(), self.works.shape[0], self.waves, self.tiles, self.base.data_ptr(), self.row_tables.data_ptr(),
-            self.rows, self.parts, self.even, self.n_heads, self.n_kv, HEAD_DIM))
+        launch = _Launch(self.works.data_ptr(), self.base.data_ptr(), self.row_tables.data_ptr(), self.works.shape[0], self.waves,
+                         self.tiles, self.rows, self.parts, self.even, self.n_heads, self.n_kv, HEAD_DIM, self.max_ctx)
+        object.__setattr__(self, "launch", launch)
+        object.__setattr__(self, "at", ctypes.addressof(launch))
 
 
 def _int(x, what: str) -> int:
@@ -300,7 +310,6 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         with torch.cuda.device(dev):
             return prefix_attention(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale)
     _lib.check(_lib.lib().p2p_prefix_attention(
-        qp, sq, kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), plan.max_ctx,
-        *plan.launch, scale, op, so, wp, wp + plan.parts * width * 4,
+        plan.at, qp, sq, kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), scale, op, so, wp,
         torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
     return out
