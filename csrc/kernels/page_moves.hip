@@ -17,7 +17,7 @@ struct Cache {   // strides in bytes
 // The pairs travel in the launch's own arguments: no copy to the device and no memory to keep until the launch has run.  A
 // workgroup takes a page of a head in a layer, 16 bytes a thread, so a token's row of any type is whole pieces.  Bound by memory:
 // 203 pages of 8 heads in 8 layers, 400 MB read and as much written, 157 us = 5.1 TB/s (a large copy has 4.9); one page in 32
-// layers is a launch of 4 us, behind 9 us of the host's.
+// layers is a launch of 4 us, behind 8 us of the host's.
 constexpr int PAIRS = 256;
 struct Pairs {
   int src[PAIRS], dst[PAIRS];

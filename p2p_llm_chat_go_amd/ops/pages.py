@@ -15,21 +15,23 @@ from .attention import HEAD_DIM, PAGE
 
 
 def _caches(k: torch.Tensor, v: torch.Tensor, what: str):
-    """Strides in bytes between layers, pages and heads of k, then of v."""
-    shape, strides = k.shape, k.stride() + v.stride()
-    if len(shape) != 5 or v.dim() != 5 or shape[3] != PAGE or shape[4] != HEAD_DIM:
+    """What the calls take of two caches: addresses, strides in bytes between layers, pages and heads of k, then of v, layers,
+    heads, pages, bytes of a token's row; and their device's index (-1: not a GPU's)."""
+    shape, strides, dev, size = k.shape, k.stride() + v.stride(), k.get_device(), k.element_size()
+    if len(shape) != 5 or len(strides) != 10 or shape[3] != PAGE or shape[4] != HEAD_DIM:
         raise ValueError("%s: k and v must be [layers, pages, kv heads, %d, %d], got %s and %s"
                          % (what, PAGE, HEAD_DIM, list(shape), list(v.shape)))
-    if shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+    if shape != v.shape or k.dtype != v.dtype or dev != v.get_device() or (dev < 0 and k.device != v.device):
         raise ValueError("%s: k and v differ in shape, type or device" % what)
-    size = k.element_size()
-    if size not in (1, 2, 4) or k.dtype.is_complex:
+    if size not in (1, 2, 4) or k.is_complex():
         raise ValueError("%s: k and v have numbers of type %s" % (what, k.dtype))
     kl, kp, kh, kt, k1, vl, vp, vh, vt, v1 = strides
-    if k1 != 1 or v1 != 1 or kt != HEAD_DIM or vt != HEAD_DIM or (kl | kp | kh | vl | vp | vh) * size % 16 \
-            or (k.data_ptr() | v.data_ptr()) % 16:
+    ka, va = k.data_ptr(), v.data_ptr()
+    if k1 != 1 or v1 != 1 or kt != HEAD_DIM or vt != HEAD_DIM or (kl | kp | kh | vl | vp | vh) * size % 16 or (ka | va) % 16:
         raise ValueError("%s: the tokens of a page must be contiguous and start at multiples of 16 bytes" % what)
-    return _SIX(kl * size, kp * size, kh * size, vl * size, vp * size, vh * size)
+    layers, pages, heads = shape[:3]
+    return (ka, va, _SIX(kl * size, kp * size, kh * size, vl * size, vp * size, vh * size), layers, heads, pages,
+            HEAD_DIM * size), dev
 
 
 _SIX = ctypes.c_long * 6
@@ -51,14 +53,14 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src, dst, tokens=None) -> None:
 
     src, dst, tokens: host numbers, as allocators give them.  tokens: how many of a page's tokens are copied (None: all); the
     others of the page stay.  A page is in dst once at most and then not in src (but ``src[i] == dst[i]`` is nothing to do)."""
-    strides = _caches(k, v, "copy_pages")
+    caches, dev = _caches(k, v, "copy_pages")
     src, dst = _ints(src, "src"), _ints(dst, "dst")
     tokens = array.array("i", [PAGE]) * len(src) if tokens is None else _ints(tokens, "tokens")
     if not len(src) == len(dst) == len(tokens):
         raise ValueError("copy_pages: %d pages to %d, %d numbers of tokens" % (len(src), len(dst), len(tokens)))
     if not src:
         return
-    P = k.shape[1]
+    P = caches[5]
     if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= P:
         raise ValueError("copy_pages: pages must be 0 .. %d" % (P - 1))
     if min(tokens) < 0 or max(tokens) > PAGE:
@@ -68,18 +70,17 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src, dst, tokens=None) -> None:
         raise ValueError("copy_pages: a page is in dst twice")
     if not to.isdisjoint(src) and not {d for s, d in zip(src, dst) if s != d}.isdisjoint(src):
         raise ValueError("copy_pages: a page is in src and in dst")
-    if k.numel() == 0:
+    if caches[3] == 0 or caches[4] == 0:
         return
-    if k.device.type != "cuda":
+    if dev < 0:
         for s, d, n in zip(src, dst, tokens):
             k[:, d, :, :n] = k[:, s, :, :n]
             v[:, d, :, :n] = v[:, s, :, :n]
         return
-    with _lib.device_of(k.get_device()):
+    with _lib.device_of(dev):
         _lib.check(_lib.lib().p2p_copy_pages(
-            k.data_ptr(), v.data_ptr(), strides, k.shape[0], k.shape[2], P, HEAD_DIM * k.element_size(),
-            src.buffer_info()[0], dst.buffer_info()[0], tokens.buffer_info()[0], len(src), _lib.stream_ptr(k.device)),
-            "copy_pages")
+            *caches, src.buffer_info()[0], dst.buffer_info()[0], tokens.buffer_info()[0], len(src),
+            torch._C._cuda_getCurrentRawStream(dev)), "copy_pages")
 
 
 def compact_pages_ref(k, v, block_tables, lens, keep, out_tables, cos_sin):
@@ -117,7 +118,7 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
     cos_sin: float32 [positions, 64, 2] (``models.config.rope_table``): keys that were rotated for position p are turned on to
     position n (bf16 caches); None: they stay as they are, as for sequences that go on counting positions.  Entries of the
     tables that are no pages are skipped."""
-    strides = _caches(k, v, "compact_pages")
+    caches, dev = _caches(k, v, "compact_pages")
     def need(ok, why):
         if not ok:
             raise ValueError("compact_pages: " + why)
@@ -141,17 +142,16 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
              "cos_sin must be float32 [%d or more, %d, 2], contiguous" % (most, HEAD_DIM // 2))
     need(all(t is None or t.device == k.device for t in (v, block_tables, lens, keep, out_tables, cos_sin)),
          "tensors must be on one device")
-    if k.device.type != "cuda":
+    if dev < 0:
         return compact_pages_ref(k, v, block_tables, lens, keep, out_tables, cos_sin)
     new = torch.empty(B, dtype=torch.int32, device=k.device)
     if B == 0:
         return new
     if k.numel() == 0 or most == 0:
         return new.copy_((keep & (torch.arange(keep.shape[1], device=k.device) < lens[:, None].clamp(max=most))).sum(1))
-    with _lib.device_of(k.get_device()):
+    with _lib.device_of(dev):
         _lib.check(_lib.lib().p2p_compact_pages(
-            k.data_ptr(), v.data_ptr(), strides, k.shape[0], k.shape[2], k.shape[1], HEAD_DIM * k.element_size(),
-            block_tables.data_ptr(), block_tables.stride(0), W, _lib.ptr(out_tables),
+            *caches, block_tables.data_ptr(), block_tables.stride(0), W, _lib.ptr(out_tables),
             0 if out_tables is None else out_tables.stride(0), lens.data_ptr(), keep.data_ptr(), keep.stride(0), keep.shape[1],
-            B, _lib.ptr(cos_sin), new.data_ptr(), _lib.stream_ptr(k.device)), "compact_pages")
+            B, _lib.ptr(cos_sin), new.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "compact_pages")
     return new
