@@ -8,7 +8,7 @@
 // be done together with other rows that see the same keys.  The host cuts the batch into works (`Work`): query rows of one
 // group (or of one sequence) against a range of pages, in `of` parts; the parts' results (fp32) meet in a second launch.
 //
-// What it takes, calls one after the other: 2 rows behind 256 tokens 7 us (the host 9), 19 behind 2048 13 and 41 on one kv head
+// What it takes, calls one after the other: 2 rows behind 256 tokens 7 us (the host 8), 19 behind 2048 13 and 41 on one kv head
 // 15, of which the second launch is 3: chains of loads of some 0.7 us each (work, page numbers, keys, values) and the launches.
 // 704 prompt rows behind 1536 tokens 34 us, 64 rows of 64 heads behind 32768 107 us: the products, see the tiles.
 #include "common.h"

@@ -277,19 +277,19 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         Ro, wo = out.shape
         tables, pages = block_tables.shape
         rows, = ctx_lens.shape
+        (sq, q1), (so, o1), (sb, b1), (c1,) = q.stride(), out.stride(), block_tables.stride(), ctx_lens.stride()
         P, h, t, d = shape = k_cache.shape
         ok = (Rq >= R and wq == wo == width and Ro >= R and tables >= plan.tables and pages * PAGE >= plan.max_ctx and rows >= R
               and shape == v_cache.shape and h == n_kv and t == PAGE and d == HEAD_DIM and P > 0
               and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16
               and block_tables.dtype == ctx_lens.dtype == torch.int32
-              and q.stride(1) == out.stride(1) == block_tables.stride(1) == ctx_lens.stride(0) == 1
+              and q1 == o1 == b1 == c1 == 1 and sq < FAR > so and sb < FAR and (so >= width or R == 1)
               and k_cache.is_contiguous() and v_cache.is_contiguous() and 0 < scale < math.inf
               and dev == out.get_device() == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
               == ctx_lens.get_device() == works.get_device())
-        kp, vp, qp, op, sq, so = k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0)
+        kp, vp, qp, op = k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr(), out.data_ptr()
         if qp + 2 * (R * sq + width) > op and op + 2 * (R * so + width) > qp:
             ok = ok and not _overlap(q, out, R, width)
-        ok = ok and (so >= width or R == 1) and sq < FAR > so and block_tables.stride(0) < FAR
         if ok and dev >= 0:
             wp = workspace.data_ptr()
             ok = ((kp | vp | wp) % 16 == 0 and workspace.get_device() == dev and workspace.dtype == torch.float32
@@ -310,6 +310,6 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         with torch.cuda.device(dev):
             return prefix_attention(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale)
     _lib.check(_lib.lib().p2p_prefix_attention(
-        plan.at, qp, sq, kp, vp, P, block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), scale, op, so, wp,
+        plan.at, qp, sq, kp, vp, P, block_tables.data_ptr(), sb, ctx_lens.data_ptr(), scale, op, so, wp,
         torch._C._cuda_getCurrentRawStream(dev)), "prefix_attention")
     return out
