@@ -35,6 +35,7 @@ def _caches(k: torch.Tensor, v: torch.Tensor, what: str):
 
 
 _SIX = ctypes.c_long * 6
+FAR = 2 ** 31          # strides of tables are below
 
 
 def _ints(x, what: str) -> array.array:
@@ -107,6 +108,34 @@ def compact_pages_ref(k, v, block_tables, lens, keep, out_tables, cos_sin):
     return new
 
 
+def _refuse(k, block_tables, lens, keep, out_tables, cos_sin):
+    """Says which of compact_pages' conditions does not hold."""
+    def need(ok, why):
+        if not ok:
+            raise ValueError("compact_pages: " + why)
+    need(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and (block_tables.stride(1) == 1 or block_tables.shape[1] < 2),
+         "block_tables must be int32 [sequences, pages]")
+    B, W = block_tables.shape
+    need(lens.dim() == 1 and lens.dtype == torch.int32 and lens.shape[0] == B and (B < 2 or lens.stride(0) == 1),
+         "lens must be int32 [%d]" % B)
+    need(keep.dim() == 2 and keep.dtype == torch.bool and keep.shape[0] == B and (keep.stride(1) == 1 or keep.shape[1] < 2),
+         "keep must be bool [%d, tokens]" % B)
+    need(B <= 65535, "more than 65535 sequences")
+    if out_tables is not None:
+        need(out_tables.dtype == torch.int32 and out_tables.shape == block_tables.shape
+             and (out_tables.stride(1) == 1 or W < 2), "out_tables must be like block_tables")
+    need(all(t is None or t.stride(0) < FAR for t in (block_tables, out_tables)), "tables with rows too far apart")
+    most = min(keep.shape[1], W * PAGE)
+    if cos_sin is not None:
+        need(k.dtype == torch.bfloat16, "keys are turned in bf16 caches only, not in %s" % k.dtype)
+        need(cos_sin.dtype == torch.float32 and cos_sin.dim() == 3 and cos_sin.shape[1:] == (HEAD_DIM // 2, 2)
+             and cos_sin.is_contiguous() and cos_sin.shape[0] >= most and cos_sin.data_ptr() % 16 == 0,
+             "cos_sin must be float32 [%d or more, %d, 2], contiguous" % (most, HEAD_DIM // 2))
+    need(all(t is None or t.device == k.device for t in (block_tables, lens, keep, out_tables, cos_sin)),
+         "tensors must be on one device")
+    raise AssertionError("compact_pages: the two forms of its conditions differ")
+
+
 def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor,
                   out_tables: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None) -> torch.Tensor:
     """The kept tokens of every sequence, together and in their order: in every layer and head, token p of sequence b becomes
@@ -119,39 +148,38 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
     position n (bf16 caches); None: they stay as they are, as for sequences that go on counting positions.  Entries of the
     tables that are no pages are skipped."""
     caches, dev = _caches(k, v, "compact_pages")
-    def need(ok, why):
-        if not ok:
-            raise ValueError("compact_pages: " + why)
-    need(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and (block_tables.stride(1) == 1 or block_tables.shape[1] < 2),
-         "block_tables must be int32 [sequences, pages]")
-    B, W = block_tables.shape
-    need(lens.dim() == 1 and lens.dtype == torch.int32 and lens.shape[0] == B and (B < 2 or lens.stride(0) == 1),
-         "lens must be int32 [%d]" % B)
-    need(keep.dim() == 2 and keep.dtype == torch.bool and keep.shape[0] == B and (keep.stride(1) == 1 or keep.shape[1] < 2),
-         "keep must be bool [%d, tokens]" % B)
-    need(B <= 65535, "more than 65535 sequences")
-    need(all(t is None or t.stride(0) < 2 ** 31 for t in (block_tables, out_tables)), "tables with rows too far apart")
-    if out_tables is not None:
-        need(out_tables.dtype == torch.int32 and out_tables.shape == block_tables.shape
-             and (out_tables.stride(1) == 1 or W < 2), "out_tables must be like block_tables")
-    most = min(keep.shape[1], W * PAGE)
-    if cos_sin is not None:
-        need(k.dtype == torch.bfloat16, "keys are turned in bf16 caches only, not in %s" % k.dtype)
-        need(cos_sin.dtype == torch.float32 and cos_sin.dim() == 3 and cos_sin.shape[1:] == (HEAD_DIM // 2, 2)
-             and cos_sin.is_contiguous() and cos_sin.shape[0] >= most and cos_sin.data_ptr() % 16 == 0,
-             "cos_sin must be float32 [%d or more, %d, 2], contiguous" % (most, HEAD_DIM // 2))
-    need(all(t is None or t.device == k.device for t in (v, block_tables, lens, keep, out_tables, cos_sin)),
-         "tensors must be on one device")
+    try:
+        (B, W), (n,), (rows, places) = block_tables.shape, lens.shape, keep.shape
+        (sb, b1), (l1,), (sk, k1) = block_tables.stride(), lens.stride(), keep.stride()
+        most = min(places, W * PAGE)
+        ok = (n == rows == B <= 65535 and block_tables.dtype == lens.dtype == torch.int32 and keep.dtype == torch.bool
+              and (b1 == 1 or W < 2) and (l1 == 1 or B < 2) and (k1 == 1 or places < 2) and sb < FAR
+              and dev == block_tables.get_device() == lens.get_device() == keep.get_device())
+        st = 0
+        if ok and out_tables is not None:
+            st, t1 = out_tables.stride()
+            ok = (out_tables.dtype == torch.int32 and out_tables.shape == (B, W) and (t1 == 1 or W < 2) and st < FAR
+                  and dev == out_tables.get_device())
+        if ok and cos_sin is not None:
+            positions, half, two = cos_sin.shape
+            ok = (k.dtype == torch.bfloat16 and cos_sin.dtype == torch.float32 and half == HEAD_DIM // 2 and two == 2
+                  and positions >= most and cos_sin.is_contiguous() and cos_sin.data_ptr() % 16 == 0
+                  and dev == cos_sin.get_device())
+        if ok and dev < 0:
+            ok = all(t is None or t.device == k.device for t in (block_tables, lens, keep, out_tables, cos_sin))
+    except ValueError:       # another number of dimensions
+        ok = False
+    if not ok:
+        _refuse(k, block_tables, lens, keep, out_tables, cos_sin)
     if dev < 0:
         return compact_pages_ref(k, v, block_tables, lens, keep, out_tables, cos_sin)
     new = torch.empty(B, dtype=torch.int32, device=k.device)
     if B == 0:
         return new
-    if k.numel() == 0 or most == 0:
-        return new.copy_((keep & (torch.arange(keep.shape[1], device=k.device) < lens[:, None].clamp(max=most))).sum(1))
+    if most == 0 or 0 in k.shape:
+        return new.copy_((keep & (torch.arange(places, device=k.device) < lens[:, None].clamp(max=most))).sum(1))
     with _lib.device_of(dev):
         _lib.check(_lib.lib().p2p_compact_pages(
-            *caches, block_tables.data_ptr(), block_tables.stride(0), W, _lib.ptr(out_tables),
-            0 if out_tables is None else out_tables.stride(0), lens.data_ptr(), keep.data_ptr(), keep.stride(0), keep.shape[1],
-            B, _lib.ptr(cos_sin), new.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "compact_pages")
+            *caches, block_tables.data_ptr(), sb, W, _lib.ptr(out_tables), st, lens.data_ptr(), keep.data_ptr(), sk, places, B,
+            _lib.ptr(cos_sin), new.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "compact_pages")
     return new

@@ -170,6 +170,10 @@ def test_nothing_to_copy():
     ("bf16 caches only", dict(cos_sin=torch.zeros(200, 64, 2))),
     ("cos_sin", dict(bf=True, cos_sin=torch.zeros(99, 64, 2))), ("cos_sin", dict(bf=True, cos_sin=torch.zeros(200, 64, 2, dtype=BF))),
     ("one device", dict(lens=torch.zeros(2, dtype=torch.int32, device="meta"))),
+    ("block_tables", dict(block_tables=torch.zeros(3, 2, dtype=torch.int32).t())), ("block_tables", dict(block_tables=torch.zeros(2, dtype=torch.int32))),
+    ("too far", dict(block_tables=torch.ones(1, dtype=torch.int32, device="meta").as_strided((2, 3), (2 ** 31, 1)))),
+    ("out_tables", dict(out_tables=torch.zeros(2, dtype=torch.int32))), ("out_tables", dict(out_tables=torch.zeros(2, 3))),
+    ("cos_sin", dict(bf=True, cos_sin=torch.zeros(200, 128))), ("cos_sin", dict(bf=True, cos_sin=torch.zeros(200, 64, 4)[..., ::2])),
 ])
 def test_compaction_that_is_refused(why, kw):
     a = dict(block_tables=torch.ones(2, 3, dtype=torch.int32), lens=torch.ones(2, dtype=torch.int32),
