@@ -112,43 +112,60 @@ class _Shape:
                 count[a:a + n] = [count[a] + C] * n
         return works, count
 
-    def micros(self, waves: int, share: bool, shared_parts: int, own_parts: int) -> float:
+    def _sizes(self, share: bool, shared_parts: int, own_parts: int):
+        """Workgroups and the longest one's pages of tiles of up to 128 pairs, of up to 32 pairs (in units of two pages), parts of
+        all rows, pages of the batch and pages that workgroups load."""
+        many = few = many_pages = few_units = parts = read = loaded = 0
+        for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
+            # contexts end somewhere up to the plan's longest: half of the pages on average, some tokens more in the longest
+            rest = self.pages - p
+            own = (rest + 1) // 2
+            longest = own + 4 if own + 4 < rest else rest
+            read += p + runs * own
+            if share and p:
+                C = (p + 1) // 2
+                if shared_parts < C:
+                    C = shared_parts
+                parts += rows * C
+                loaded += tiles * p
+                if tiles_many:
+                    many += tiles * C
+                    many_pages = max(many_pages, -(-p // C))
+                else:
+                    few += tiles * C
+                    few_units = max(few_units, -(-p // (2 * C)))
+                C = (rest + 1) // 2
+            else:
+                own, longest, C = p + own, self.pages, (self.pages + 1) // 2
+            if own_parts < C:
+                C = own_parts
+            if C:
+                parts += rows * C
+                loaded += runs * own
+                if runs_many:
+                    many += runs * C
+                    many_pages = max(many_pages, -(-longest // C))
+                else:
+                    few += runs * C
+                    few_units = max(few_units, -(-longest // (2 * C)))
+        return many * self.n_kv, many_pages, few * self.n_kv, few_units, parts, read, loaded
+
+    def micros(self, waves: int, share: bool, sizes) -> float:
         """About how long a call takes: constants fitted to timings of 78 batches, of 2 to 768 rows behind 128 to 32768 tokens, cut
         in all ways.  A launch and its first loads 4.1 us (of 8 wavefronts 5.2); a page of a tile of 128 pairs 1.25 us where CUs
         have one workgroup, 1.4 where they have two, two pages of 8 wavefronts 2.25; 32 keys of a wavefront 0.65 (0.8); what memory
         and L2 add, as if they were three sides of a box, at 17.5 and 25 TB/s (the caches held much of it); a second launch 2.1,
         0.84 per MB of the parts' results; rows alone in parts a twentieth more.  The cut that it puts first takes 2.4 % longer
         than the fastest one on average."""
-        many = few = many_pages = few_units = parts = read = loaded = 0
-        for p, tiles, tiles_many, runs, runs_many, rows in self.sums:
-            # contexts end somewhere up to the plan's longest: half of the pages on average, some tokens more in the longest
-            own = (self.pages - p + 1) // 2
-            longest = min(self.pages - p, own + 4)
-            read += p + runs * own
-            if share and p:
-                todo = ((tiles, tiles_many, p, p, min(shared_parts, -(-p // 2))),
-                        (runs, runs_many, own, longest, min(own_parts, -(-longest // 2))))
-            else:
-                todo = ((runs, runs_many, p + own, self.pages, min(own_parts, -(-self.pages // 2))),)
-            for n, is_many, pages, most_pages, C in todo:
-                if not C:
-                    continue
-                parts += rows * C
-                loaded += n * pages
-                if is_many:
-                    many += n * C * self.n_kv
-                    many_pages = max(many_pages, -(-most_pages // C))
-                else:
-                    few += n * C * self.n_kv
-                    few_units = max(few_units, -(-most_pages // (2 * C)))
-        eight, most = waves == 8, 2048 // waves        # (workgroups at once)
-        if eight:
-            many_pages, few_units = -(-many_pages // 2), -(-few_units // 2)
-        t_many = many_pages * (2.25 if eight else 1.25 if many <= 256 else 1.4) * -(-many // most)
-        t_few = few_units * (0.8 if eight else 0.65) * -(-few // most)
-        t = max(t_many, t_few) if many + few <= most else t_many + t_few
-        page = self.n_kv * 32768e-6                    # MB
-        t = (5.2 if eight else 4.1) + math.hypot(t, read * page / 17.5, loaded * page / 25)
+        many, many_pages, few, few_units, parts, read, loaded = sizes
+        if waves == 8:
+            t, most, page, unit = 5.2, 256, 2.25, 0.8       # (most: workgroups at once)
+            many_pages, few_units = (many_pages + 1) // 2, (few_units + 1) // 2
+        else:
+            t, most, page, unit = 4.1, 512, 1.25 if many <= 256 else 1.4, 0.65
+        t_many, t_few = many_pages * page * -(-many // most), few_units * unit * -(-few // most)
+        mb = self.n_kv * 32768e-6                      # of a page
+        t += math.hypot(max(t_many, t_few) if many + few <= most else t_many + t_few, read * mb / 17.5, loaded * mb / 25)
         if parts > self.R:
             t += 2.1 + 0.84e-6 * parts * self.n_heads * 512
             if not share:
@@ -160,11 +177,17 @@ class _Shape:
         upto = lambda parts, pages: [c for c in parts if c == 1 or c <= -(-pages // 2)]
         most = max(p for p, _t, _r in self.groups)
         least = min(p for p, _t, _r in self.groups)
-        ways = [(waves, False, 1, own) for waves in (4, 8) for own in upto(OWN_PARTS, self.pages)]
+        cuts = [(False, 1, own) for own in upto(OWN_PARTS, self.pages)]
         if most:
-            ways += [(waves, True, shared, own) for waves in (4, 8) for shared in upto(SHARED_PARTS, most)
-                     for own in upto(OWN_PARTS, self.pages - least)]
-        return min(ways, key=lambda way: self.micros(*way))
+            cuts += [(True, shared, own) for shared in upto(SHARED_PARTS, most) for own in upto(OWN_PARTS, self.pages - least)]
+        best = math.inf
+        for cut in cuts:
+            sizes = self._sizes(*cut)
+            for waves in (4, 8):
+                t = self.micros(waves, cut[0], sizes)
+                if t < best:
+                    best, way = t, (waves, *cut)
+        return way
 
 
 def prefix_plan(groups, n_heads: int, n_kv: int, max_ctx: int, device, seqs=None) -> PrefixPlan:
