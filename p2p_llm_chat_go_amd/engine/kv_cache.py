@@ -125,6 +125,8 @@ class KVCache:
         if any(n < need for n in sizes):
             raise ValueError("fork: %d tokens take %d pages, asked for %d" % (tokens, need, min(sizes)))
         self.allocator.check(pages[:need])
+        if len(set(pages[:need])) < need:
+            raise ValueError("fork: a page is given twice")
         fresh = self.allocator.alloc(sum(n - full for n in sizes))
         out, at = [], 0
         for n in sizes:
@@ -153,7 +155,7 @@ class KVCache:
             raise ValueError("compact: room for %d tokens" % room)
         given = collections.Counter(p for q in pages for p in q)
         self.allocator.check(given)
-        if any(n > self.allocator.owners(p) for p, n in given.items()):
+        if any(len(set(q)) < len(q) for q in pages) or any(n > self.allocator.owners(p) for p, n in given.items()):
             raise ValueError("compact: a page is given twice, or by more sequences than own it")
         if not pages:
             return [], []

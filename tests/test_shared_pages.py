@@ -143,6 +143,23 @@ def test_compactions_that_are_refused():
     assert kv.allocator.free_pages == 7
 
 
+def test_a_page_twice_in_one_sequence_is_refused():
+    """Two owners of a page are two sequences: one that lists it twice would give up the other's, too."""
+    kv = _cache("cpu", 8)
+    a = kv.allocator.alloc(2)
+    b, = kv.fork(a, 128, [2])
+    keep = torch.ones(2, 128, dtype=torch.bool)
+    for pages, lens in (([[a[0], a[0]]], [128]), ([a, [b[1], b[1]]], [128, 9])):
+        with pytest.raises(ValueError, match="given twice"):
+            kv.compact(pages, lens, keep[:len(pages)])
+    with pytest.raises(ValueError, match="given twice"):
+        kv.fork([a[0], a[0]], 128, [2])
+    assert kv.allocator.free_pages == 5 and all(kv.allocator.owners(p) == 2 for p in a)
+    kv.allocator.free(a)
+    kv.allocator.free(b)
+    assert sorted(kv.allocator.alloc(7)) == list(range(1, 8))
+
+
 def test_common_prefixes():
     assert common_prefix([[1, 2, 3], (1, 2, 3, 4)]) == 2
     assert common_prefix([[1, 2, 3], [1, 2, 4, 5]]) == 2 and common_prefix([[1, 2, 3], [1, 2, 3]]) == 2
