@@ -34,7 +34,7 @@ class PageAllocator:
             raise ValueError("need at least 2 pages (page 0 is the null page)")
         self.num_pages = num_pages
         self._free = list(range(num_pages - 1, 0, -1))
-        self._more = {}      # page -> owners beyond the first
+        self._owners = [0] * num_pages      # of every page; 0: free
 
     @property
     def free_pages(self) -> int:
@@ -42,40 +42,44 @@ class PageAllocator:
 
     def shared(self, page: int) -> bool:
         """Whether more than one sequence owns the page."""
-        return page in self._more
+        return self._owners[page] > 1
 
     def owners(self, page: int) -> int:
-        """How many sequences own a page that is in use."""
-        return 1 + self._more.get(page, 0)
+        """How many sequences own a page (0: it is free)."""
+        return self._owners[page]
 
     def check(self, pages):
-        """Raises where one of them is no page that a sequence can own."""
+        """Raises where one of them is no page that a sequence can own, or free."""
         for p in pages:
             if p <= 0 or p >= self.num_pages:
                 raise ValueError("bad page %d" % p)
+            if not self._owners[p]:
+                raise ValueError("page %d is free" % p)
 
     def share(self, pages):
         """One more owner for each of the pages (which are in use); each owner frees them once."""
         self.check(pages)
         for p in pages:
-            self._more[p] = self._more.get(p, 0) + 1
+            self._owners[p] += 1
 
     def alloc(self, n: int) -> list:
         if n > len(self._free):
             raise MemoryError("KV cache exhausted: want %d pages, %d free" % (n, len(self._free)))
         out = [self._free.pop() for _ in range(n)]
+        for p in out:
+            self._owners[p] = 1
         return out
 
     def free(self, pages):
+        """Each of the pages loses an owner; nothing has changed where one of them cannot."""
         self.check(pages)
+        for p, n in collections.Counter(pages).items():
+            if n > self._owners[p]:
+                raise ValueError("page %d is freed more often than it is owned" % p)
         for p in pages:
-            more = self._more.get(p)
-            if more is None:
+            self._owners[p] -= 1
+            if not self._owners[p]:
                 self._free.append(p)
-            elif more == 1:
-                del self._more[p]
-            else:
-                self._more[p] = more - 1
 
 
 def pages_for(tokens: int) -> int:

@@ -143,6 +143,29 @@ def test_compactions_that_are_refused():
     assert kv.allocator.free_pages == 7
 
 
+def test_pages_that_nobody_owns_are_refused():
+    """A page that is free is not shared, forked, compacted or freed once more: it would be handed out while it is held."""
+    kv = _cache("cpu", 8)
+    a = kv.allocator
+    one, = a.alloc(1)
+    assert a.owners(one) == 1
+    a.free([one])
+    assert a.owners(one) == 0
+    keep = torch.ones(1, 64, dtype=torch.bool)
+    for call in (lambda: a.share([one]), lambda: kv.fork([one], 64, [2]), lambda: kv.compact([[one]], [64], keep),
+                 lambda: a.free([one])):
+        with pytest.raises(ValueError, match="page %d is free" % one):
+            call()
+        assert a.free_pages == 7 and not a.shared(one)
+    two = a.alloc(2)
+    with pytest.raises(ValueError, match="more often than"):      # nothing is freed where one of them cannot be
+        a.free([two[1], two[0], two[0]])
+    assert a.free_pages == 5
+    a.share(two[:1])
+    a.free([two[0], two[0], two[1]])
+    assert sorted(a.alloc(7)) == list(range(1, 8))
+
+
 def test_a_page_twice_in_one_sequence_is_refused():
     """Two owners of a page are two sequences: one that lists it twice would give up the other's, too."""
     kv = _cache("cpu", 8)
