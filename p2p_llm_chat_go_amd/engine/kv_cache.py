@@ -131,6 +131,7 @@ class KVCache:
         self.allocator.check(pages[:need])
         if len(set(pages[:need])) < need:
             raise ValueError("fork: a page is given twice")
+        copy_pages(self.k, self.v, [], [])      # what the copies would refuse: nothing has changed yet
         fresh = self.allocator.alloc(sum(n - full for n in sizes))
         out, at = [], 0
         for n in sizes:

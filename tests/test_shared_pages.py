@@ -143,6 +143,14 @@ def test_compactions_that_are_refused():
     assert kv.allocator.free_pages == 7
 
 
+def test_a_fork_whose_copy_is_refused_takes_no_pages():
+    kv = KVCache(TINY_LLAMA, 8, "cpu", dtype=torch.float64)      # a type that copies do not take
+    mine = kv.allocator.alloc(2)
+    with pytest.raises(ValueError, match="float64"):
+        kv.fork(mine, 100, [2])
+    assert kv.allocator.free_pages == 5 and not kv.allocator.shared(mine[0])
+
+
 def test_pages_that_nobody_owns_are_refused():
     """A page that is free is not shared, forked, compacted or freed once more: it would be handed out while it is held."""
     kv = _cache("cpu", 8)
