@@ -325,8 +325,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, scale)
     if dev < 0:
         ctx = ctx_lens[:R].clamp(0, plan.max_ctx)
-        paged_attention_ref(q[:R], k_cache, v_cache, block_tables, plan.row_tables, ctx.clamp(min=1), n_heads, n_kv, scale,
-                            out[:R])
+        paged_attention_ref(q[:R], k_cache, v_cache, block_tables.clamp(0, P - 1), plan.row_tables, ctx.clamp(min=1), n_heads,
+                            n_kv, scale, out[:R])
         out[:R] = torch.where((ctx > 0)[:, None], out[:R], 0)
         return out
     if dev != torch._C._cuda_getDevice():

@@ -127,6 +127,14 @@ def test_attention_on_the_cpu():
     assert bool(((out.double().view(3, 4, D) - want).abs() <= bound).all()) and bool((out[1] == 0).all())
 
 
+def test_attention_on_the_cpu_reads_entries_that_are_no_pages_inside_the_cache():
+    a = _given()
+    a["block_tables"] = torch.tensor([[1, 10 ** 9], [-7, 3], [-1, 4]], dtype=torch.int32)
+    inside = torch.tensor([[1, 8], [0, 3], [0, 4]], dtype=torch.int32)
+    want, bound = oracle.attention(a["q"], a["k_cache"], a["v_cache"], inside, [0, 1, 2], a["ctx_lens"], 4, 2, D ** -0.5, 128)
+    assert bool(((ops.prefix_attention(**a).double().view(3, 4, D) - want).abs() <= bound).all())
+
+
 def _pages(pages=8, **kw):
     return torch.zeros(2, pages, 2, PAGE, D, **kw), torch.zeros(2, pages, 2, PAGE, D, **kw)
 
