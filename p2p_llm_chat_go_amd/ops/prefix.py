@@ -22,6 +22,7 @@ SCALE = 1.0 / math.sqrt(HEAD_DIM)
 SHARED_PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96)
 OWN_PARTS = (1, 2, 4, 8, 16, 32, 64)
 FAR = 2 ** 31          # strides are below
+LEAST_SCALE, MOST_SCALE = 2.0 ** -64, 2.0 ** 64    # (the kernel's scores and their scale are fp32)
 FEW, MANY = 32, 128    # (row, head) pairs of a workgroup, in the kernel's two roles
 
 
@@ -264,7 +265,7 @@ def _refuse(q, k_cache, v_cache, block_tables, ctx_lens, plan, out, workspace, s
          "block_tables must be int32 [%d or more, pages of %d tokens]" % (plan.tables, plan.max_ctx))
     need(ctx_lens.dim() == 1 and ctx_lens.dtype == torch.int32 and ctx_lens.shape[0] >= R and ctx_lens.stride(0) == 1,
          "ctx_lens must be int32 [%d or more]" % R)
-    need(0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
+    need(LEAST_SCALE <= scale <= MOST_SCALE, "scale must be 2^-64 .. 2^64, got %r" % scale)
     need(out.dim() == 2 and out.dtype == torch.bfloat16 and out.shape[0] >= R and out.shape[1] == width and out.stride(1) == 1
          and (out.stride(0) >= width or R == 1) and out.stride(0) < FAR,
          "out must be bf16 [%d or more, %d], rows contiguous and apart" % (R, width))
@@ -284,7 +285,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     Row r attends the first ``min(ctx_lens[r], plan.max_ctx)`` tokens of its block table; a row that sees none is 0.  Rows
     behind the plan's are not read or written; out is other memory than q.  A group's shared pages are read through its
-    first row's table.  Block tables hold pages of the cache; others read page 0 or the last one."""
+    first row's table.  Block tables hold pages of the cache; others read page 0 or the last one.  scale: 2^-64 .. 2^64 (None: 128^-0.5)."""
     R, n_heads, n_kv = plan.rows, plan.n_heads, plan.n_kv
     width = n_heads * HEAD_DIM
     if scale is None:
@@ -307,7 +308,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
               and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16
               and block_tables.dtype == ctx_lens.dtype == torch.int32
               and q1 == o1 == b1 == c1 == 1 and sq < FAR > so and sb < FAR and (so >= width or R == 1)
-              and k_cache.is_contiguous() and v_cache.is_contiguous() and 0 < scale < math.inf
+              and k_cache.is_contiguous() and v_cache.is_contiguous() and LEAST_SCALE <= scale <= MOST_SCALE
               and dev == out.get_device() == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
               == ctx_lens.get_device() == works.get_device())
         kp, vp, qp, op = k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr(), out.data_ptr()

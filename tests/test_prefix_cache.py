@@ -119,6 +119,15 @@ def test_out_is_other_memory_than_q(qs, outs, ok):
             ops.prefix_attention(**a)
 
 
+@pytest.mark.parametrize("scale", [1e-46, 2.0 ** -65, 2.0 ** 65, 1e39, 1e300])
+def test_scales_that_fp32_scores_do_not_take_are_refused(scale):
+    """Scores are fp32 numbers times the scale in fp32: one that is 0 or infinite there would leave no softmax."""
+    with pytest.raises(ValueError, match="scale"):
+        ops.prefix_attention(**_given(scale=scale))
+    for fine in (2.0 ** -64, 2.0 ** 64):
+        assert bool(torch.isfinite(ops.prefix_attention(**_given(scale=fine))).all())
+
+
 def test_attention_on_the_cpu():
     a = _given()
     out = ops.prefix_attention(**a)
