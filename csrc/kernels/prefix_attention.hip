@@ -118,8 +118,9 @@ __device__ __forceinline__ long place_of(const Args& A, const Work& W, int kvh, 
   return ((long)(before + W.slot + W.part) * A.Hkv * A.G + head) * HD;
 }
 
-// One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite.  Products of tiles
-// give 0 * inf = nan to rows of the tile that do not see the value.
+// One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite (products of tiles
+// give 0 * inf = nan to rows of the tile that do not see the value), and a row without a weight: 0 where it has no key, nan
+// where all of its keys' scores are -inf.
 __device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const int* btr, int num_pages, size_t page_sz,
                            size_t head_off, int ctx, float scale_log2, int lane, float (&acc)[2]) {
   float m = -INFINITY, l = 0.f;
@@ -148,8 +149,8 @@ __device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const
       acc[1] = fmaf(pj, (float)v[1], acc[1]);
     }
   }
-  acc[0] /= l;
-  acc[1] /= l;
+  acc[0] = ctx > 0 ? acc[0] / l : 0.f;
+  acc[1] = ctx > 0 ? acc[1] / l : 0.f;
 }
 // the same for row r's head h, from the row's block table `btr`
 __device__ void exact_pair(const Args& A, const int* btr, int r, int h, int lane, float (&acc)[2]) {
@@ -162,10 +163,10 @@ __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINI
 __device__ __forceinline__ bool put_result(const Args& A, long at, f32x4 sum, float den, int r32) {
   const float by = 1.f / den;
   bf16x4 y;
-  bool bad = false;
+  bool bad = den == 0.f;   // (no key, or none of a score above -inf)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = den == 0.f ? 0.f : sum[i] * by;   // (no key, whatever the values of others are)
+    const float x = den == 0.f ? 0.f : sum[i] * by;   // (whatever the values of others are)
     bad |= not_finite(x);
     y[i] = f2bf(x);
   }
@@ -684,9 +685,9 @@ __global__ __launch_bounds__(256) void prefix_combine_kernel(Args A, const int* 
       acc += so[x][r32] * e;
     }
   }
-  const float by = den == 0.f ? 0.f : 1.f / den;   // (0: no key)
+  const float by = den == 0.f ? 0.f : 1.f / den;   // (0: no key, or none of a score above -inf)
   bf16x4 y;
-  bool bad = false;
+  bool bad = den == 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float x = acc[i] * by;

@@ -167,6 +167,34 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(way, token
     assert float(far.max()) <= 0
 
 
+def _same_nan(got, want, bound):
+    """Equal where they are not finite, else within the bound."""
+    got = got.double().cpu().view(want.shape)
+    assert torch.equal(torch.isnan(want), torch.isnan(got)), (torch.isnan(want) != torch.isnan(got)).nonzero()[:5]
+    far = torch.where(got == want, 0, (got - want).abs() - bound).nan_to_num()
+    assert float(far.max()) <= 0, (float(far.max()), (far > 0).nonzero()[:5])
+
+
+def test_rows_whose_scores_are_all_minus_infinity_are_nan(way):
+    """No key has a weight then, as the softmax of the formula has it; rows without a key are 0."""
+    q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 4)
+    q[:, 3::D] = q[:, 3::D].abs() + 0.1
+    k[table[0, 0], 0, 0, 3] = -INF             # the first group's first key
+    k[table[12, 0], 1, :, 3] = -INF            # and all of the second group's shared ones
+    ctx[2], ctx[5], ctx[12], ctx[13], ctx[14] = 1, 0, 64, 40, 65
+    for c in (k, v):
+        c[table[14, 1], :, 0] = 0.25
+    plan = ops.prefix_plan(rows, 8, 2, most, DEV)
+    want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 2, 1 / math.sqrt(D), most)
+    # The bound's part of the scores is infinite for rows that see an infinite key: theirs is a rounding of the result and one of
+    # every weight, U16 of the largest value each, and fp32 scores of up to 60 (2 D U32 60 = 0.24 U16)
+    bound = torch.where(torch.isfinite(bound), bound, 2.5 * oracle.U16 * float(v.float().nan_to_num(0).abs().max()))
+    assert torch.isnan(want).all(-1).nonzero().tolist() == [[2, h] for h in range(4)] + [[r, h] for r in (12, 13) for h in range(4, 8)]
+    got = _run(q, k, v, table, ctx, plan)
+    _same_nan(got, want, bound)
+    assert bool((got[5] == 0).all())
+
+
 def test_rows_and_tables_of_any_stride_and_rows_behind_the_plan(way):
     q, k, v, table, seqs, ctx, rows, most = _batch([(9, 2)], 8, 2, 50, 9)
     wide = torch.randn(12, 8 * D + 3).bfloat16()
