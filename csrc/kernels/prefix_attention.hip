@@ -120,7 +120,8 @@ __device__ __forceinline__ long place_of(const Args& A, const Work& W, int kvh, 
 
 // One (row, head) pair of a wavefront, key by key in fp32: what a row sees of values that are not finite (products of tiles
 // give 0 * inf = nan to rows of the tile that do not see the value), and a row without a weight: 0 where it has no key, nan
-// where all of its keys' scores are -inf.
+// where all of its keys' scores are -inf.  Weights are 2^-32 of what they are elsewhere: sums of finite values, up to 2^32 of the
+// largest, stay finite, and what falls below 2^-126 is 2^-94 of the largest weight at most.
 __device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const int* btr, int num_pages, size_t page_sz,
                            size_t head_off, int ctx, float scale_log2, int lane, float (&acc)[2]) {
   float m = -INFINITY, l = 0.f;
@@ -136,7 +137,7 @@ __device__ void exact_pair(const bf16* qp, const bf16* kc, const bf16* vc, const
     }
     const float mn = fmaxf(m, wave_max(s));
     const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-    const float p = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);
+    const float p = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn) * 0x1p-32f;
     m = mn;
     l = fmaf(l, alpha, wave_sum(p));
     acc[0] *= alpha;

@@ -195,6 +195,18 @@ def test_rows_whose_scores_are_all_minus_infinity_are_nan(way):
     assert bool((got[5] == 0).all())
 
 
+def test_values_near_the_type_s_largest(way):
+    """Weights sum to 1: a result is no larger than its values, whatever the sums before the division are."""
+    q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 5)
+    v[..., 5] = torch.where(torch.isnan(v[..., 5]), v[..., 5], torch.tensor(3e38).bfloat16())
+    v[..., 9] = v[..., 9] * 2.0 ** 124
+    q = q * 0.1                                # weights that are near one another
+    plan = ops.prefix_plan(rows, 8, 2, most, DEV)
+    want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 2, 1 / math.sqrt(D), most)
+    assert bool(torch.isfinite(want).all())
+    _check(_run(q, k, v, table, ctx, plan), want, bound)
+
+
 def test_rows_and_tables_of_any_stride_and_rows_behind_the_plan(way):
     q, k, v, table, seqs, ctx, rows, most = _batch([(9, 2)], 8, 2, 50, 9)
     wide = torch.randn(12, 8 * D + 3).bfloat16()
