@@ -175,6 +175,23 @@ def _same_nan(got, want, bound):
     assert float(far.max()) <= 0, (float(far.max()), (far > 0).nonzero()[:5])
 
 
+def test_scores_that_are_nan_make_their_rows_nan(way):
+    """A query with a nan; a row whose last key, alone in its part, its page or its 32 keys, is nan."""
+    q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 3)
+    q[3, 5 * D + 7] = NAN
+    for r, at in ((7, 128), (8, 160), (13, 64), (14, 96), (15, 127)):     # the last key that the row sees
+        page, ctx[r] = table[r, at // PAGE], at + 1
+        for c in (k, v):
+            c[page, :, :at % PAGE] = c[page, :, :at % PAGE].nan_to_num(0.5)
+            c[page, :, at % PAGE] = 0.25
+        k[page, 1, at % PAGE] = NAN
+    plan = ops.prefix_plan(rows, 8, 2, most, DEV)
+    want, bound = oracle.attention(q, k, v, table, seqs, ctx, 8, 2, 1 / math.sqrt(D), most)
+    nan = torch.isnan(want).all(-1)
+    assert nan[3].nonzero()[:, 0].tolist() == [5] and nan[[7, 8, 13, 14, 15]].sum(0).tolist() == [0] * 4 + [5] * 4 and nan.sum() == 21
+    _same_nan(_run(q, k, v, table, ctx, plan), want, bound)
+
+
 def test_rows_whose_scores_are_all_minus_infinity_are_nan(way):
     """No key has a weight then, as the softmax of the formula has it; rows without a key are 0."""
     q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 4)
@@ -377,6 +394,49 @@ def test_compaction(apart, turn, lens, share):
     kc, vc = k.clone(), v.clone()                        # the CPU's own
     assert ops.compact_pages(kc, vc, table, n, keep, out_tables=to if apart else None, cos_sin=rot).tolist() == want_n
     assert torch.equal(vc.double(), want_v) and bool(((kc.double() - want_k).abs() <= bound).all())
+
+
+def _filled(shape, dtype, seed):
+    if dtype == torch.uint8:
+        return _caches(shape, dtype, seed)
+    return [torch.randn(shape, generator=torch.Generator().manual_seed(seed + i)).to(dtype) for i in range(2)]
+
+
+def _compacted_as(k, v, part, table, n, keep, to, rot):
+    """Compaction of ``part`` of two caches on the GPU against the oracle's; the rest of them stays."""
+    kd, vd = k.to(DEV), v.to(DEV)
+    a, b, want_n, bound = oracle.compacted(part(k), part(v), table, n, keep, to, rot)
+    got = ops.compact_pages(part(kd), part(vd), table.to(DEV), n.to(DEV), keep.to(DEV), out_tables=None if to is None else to.to(DEV),
+                            cos_sin=None if rot is None else rot.to(DEV))
+    assert got.tolist() == want_n
+    kc, vc = kd.cpu(), vd.cpu()
+    assert torch.equal(part(vc).double(), b) and bool(((part(kc).double() - a).abs() <= bound).all())
+    part(kc).copy_(part(k))
+    part(vc).copy_(part(v))
+    assert torch.equal(kc, k) and torch.equal(vc, v)
+
+
+@pytest.mark.parametrize("heads", [8, 7])      # pairs of heads of a workgroup, one head
+@pytest.mark.parametrize("dtype,turn", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.uint8, False), (torch.float32, False)])
+def test_compaction_in_place_of_many_layers_and_heads(heads, dtype, turn):
+    """16 layers and 3 sequences: two heads for a workgroup where they are even; heads 1 .. of a wider cache."""
+    table, _to, n, keep = _sequences([300, 7, 129], 17, 0.6)
+    keep[0, :70] = True
+    k, v = _filled((16, 17, heads + 2, PAGE, D), dtype, 3)
+    assert 16 * 8 * 3 >= 384      # where pairs begin
+    _compacted_as(k, v, lambda c: c[:, :, 1:1 + heads], table, n, keep, None, ROT if turn else None)
+
+
+@pytest.mark.parametrize("lens", [[2000, 700, 1500, 900], [620, 610, 600]])
+@pytest.mark.parametrize("dtype,turn", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.uint8, False), (torch.float32, False)])
+def test_compaction_into_other_pages_of_many_layers_and_heads(lens, dtype, turn):
+    """15 pairs of a layer and a head in fewer shares: a workgroup moves its tokens in several pairs, not equally many in each."""
+    table, to, n, keep = _sequences(lens, 19, 0.5)
+    chunks = -(-min(keep.shape[1], table.shape[1] * PAGE) // {1: 64, 2: 32, 4: 16}[dtype.itemsize])
+    shares = max(1, min(15, 256 // (chunks * len(lens))))
+    assert shares < 15 and (shares == 1 or 15 % shares)
+    k, v = _filled((5, 1 + 2 * table.numel(), 4, PAGE, D), dtype, 5)
+    _compacted_as(k, v, lambda c: c[:, :, :3], table, n, keep, to, ROT if turn else None)
 
 
 @pytest.mark.parametrize("apart", [False, True])
