@@ -147,9 +147,13 @@ class KVCache:
         keeps: (page lists, lengths) of what is left, with pages for ``room`` more tokens each.
 
         A sequence whose pages are its own is compacted in place, one that shares pages with others (``fork``) into new
-        ones; pages that nobody owns any more are free.  cos_sin (``LlamaModel.rope``): keys are turned to their new
-        positions, and the sequence goes on at its new length; None: it goes on counting from where it was, and only the
-        cache's places change."""
+        ones; pages that nobody owns any more are free.
+
+        cos_sin (``LlamaModel.rope``): keys are turned to their new positions, and the sequence goes on at its new length:
+        ``Engine.prefill`` (starts) and decode steps, which take a token's rotation, slot and context from one position, need
+        it so.  None: keys stay as they are; the next tokens' rotations count on from the old length while their slots and
+        contexts count from the new one, which ``LlamaModel.forward`` takes apart (pos; slots, ctx_lens) and the engine's
+        calls do not."""
         keep = torch.as_tensor(keep, dtype=torch.bool)
         if keep.dim() != 2 or keep.shape[0] != len(pages) or len(lens) != len(pages):
             raise ValueError("compact: %d sequences, %d lengths, keep %s" % (len(pages), len(lens), list(keep.shape)))

@@ -6,7 +6,7 @@ from p2p_llm_chat_go_amd import ops
 from p2p_llm_chat_go_amd.engine import Engine
 from p2p_llm_chat_go_amd.engine.engine import common_prefix
 from p2p_llm_chat_go_amd.engine.kv_cache import KVCache, PageAllocator, pages_for
-from p2p_llm_chat_go_amd.models import TINY_LLAMA
+from p2p_llm_chat_go_amd.models import LLAMA31_8B, TINY_LLAMA
 from p2p_llm_chat_go_amd.models.config import rope_table
 from p2p_llm_chat_go_amd.models.reference import random_state_dict
 from p2p_llm_chat_go_amd.models.weights import EngineWeights
@@ -119,6 +119,38 @@ def test_compaction_leaves_the_pages_of_others_alone(device, turn):
     for p in pages + [d]:
         kv.allocator.free(p)
     assert kv.allocator.free_pages == 23 and free < 23
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cfg", [TINY_LLAMA, LLAMA31_8B], ids=lambda c: c.name)
+def test_turned_keys_are_the_keys_that_the_model_rotates_for_the_new_places(device, cfg):
+    """``ops.rope_cache`` for the old positions and compaction, against ``ops.rope_cache`` for the new ones."""
+    n, KV, rot = 300, 2, rope_table(cfg, max_pos=320)
+    g = torch.Generator().manual_seed(9)
+    qkv = torch.randn(n, (2 + 2 * KV) * 128, generator=g).bfloat16()
+    keep = torch.rand(1, n, generator=g) < 0.5
+    keep[0, :3] = True
+    left = int(keep.sum())
+    table = (torch.randperm(5, generator=g) + 1).to(torch.int32)
+    slots = lambda m: (table[torch.arange(m) // PAGE] * PAGE + torch.arange(m) % PAGE).int()
+    def rotated(rows):
+        m = len(rows)
+        k, v = (torch.zeros(6, KV, PAGE, 128, dtype=torch.bfloat16, device=device) for _ in range(2))
+        ops.rope_cache(rows.to(device), torch.arange(m, dtype=torch.int32, device=device), slots(m).to(device), rot.to(device), 2, KV,
+                       torch.empty(m, 256, dtype=torch.bfloat16, device=device), k, v)
+        return k[None], v[None]
+    k, v = rotated(qkv)
+    before = _tokens(k, table.tolist(), n)[:, :, keep[0]].double()
+    assert ops.compact_pages(k, v, table[None].to(device), torch.tensor([n], dtype=torch.int32, device=device), keep.to(device),
+                             cos_sin=rot.to(device)).tolist() == [left]
+    want_k, want_v = (_tokens(c, table.tolist(), left).double() for c in rotated(qkv[keep[0]]))
+    got = _tokens(k, table.tolist(), left).double()
+    # old keys rounded (half a step of both numbers of a pair), the turned and the wanted ones rounded; products in fp32
+    x1, x2 = before.abs().chunk(2, -1)
+    pair = (x1 + x2).repeat(1, 1, 1, 2)
+    bound = oracle.U16 * (pair + got.abs() + want_k.abs()) + 24 * oracle.U32 * pair
+    assert bool(((got - want_k).abs() <= bound).all())
+    assert torch.equal(_tokens(v, table.tolist(), left).double(), want_v)
 
 
 def test_compactions_that_are_refused():
@@ -245,6 +277,78 @@ def test_prompts_over_shared_pages_have_the_logits_of_prompts_of_their_own(devic
         eng.prefill(prompts, b, starts=[150, 100, 150], shared_pages=2)
     with pytest.raises(ValueError, match="shared pages"):
         eng.prefill(prompts, b, shared_pages=2)
+
+
+def _forward_without(sd, cfg, tokens, gone, n):
+    """fp32 logits of a causal forward, where tokens from n on do not see those of ``gone`` (the ones before n do)."""
+    T, D, H, KV = len(tokens), cfg.head_dim, cfg.n_heads, cfg.n_kv_heads
+    cs = rope_table(cfg, max_pos=T)
+    cos, sin = cs[..., 0][:, None], cs[..., 1][:, None]
+    unseen = torch.ones(T, T, dtype=torch.bool).triu(1)
+    unseen[n:, gone] = True
+    x = sd["model.embed_tokens.weight"].float()[torch.tensor(tokens)]
+    norm = lambda x, w: x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + cfg.eps) * w.float()
+    turn = lambda x: torch.cat([x[..., :D // 2] * cos - x[..., D // 2:] * sin, x[..., D // 2:] * cos + x[..., :D // 2] * sin], -1)
+    for i in range(cfg.n_layers):
+        w = lambda name: sd["model.layers.%d.%s.weight" % (i, name)].float()
+        h = norm(x, w("input_layernorm"))
+        q, k, v = ((h @ w("self_attn.%s_proj" % c).t()).view(T, m, D) for c, m in (("q", H), ("k", KV), ("v", KV)))
+        k, v = (t.repeat_interleave(H // KV, 1).transpose(0, 1) for t in (turn(k), v))
+        s = (turn(q).transpose(0, 1) @ k.transpose(1, 2).contiguous() / D ** 0.5).masked_fill(unseen, -float("inf"))
+        x = x + (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(T, -1) @ w("self_attn.o_proj").t()
+        h = norm(x, w("post_attention_layernorm"))
+        x = x + (torch.nn.functional.silu(h @ w("mlp.gate_proj").t()) * (h @ w("mlp.up_proj").t())) @ w("mlp.down_proj").t()
+    x = norm(x, sd["model.norm.weight"])
+    return x @ sd["model.embed_tokens.weight" if cfg.tie_embeddings else "lm_head.weight"].float().t()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("share", [False, True])
+def test_a_sequence_goes_on_behind_a_compaction(device, share):
+    """With its keys turned by the engine's calls, at its new length; with its keys as they are by ``LlamaModel.forward``, whose
+    positions count on while slots and lengths are the compacted ones."""
+    cfg = TINY_LLAMA
+    sd = random_state_dict(cfg, seed=4)
+    for name in sd:     # attention that tells places and tokens apart: keys that were not turned are 3e-2 off, those of gone tokens 6e-2
+        sd[name] = sd[name] * (4 if "q_proj" in name else 8 if "v_proj" in name else 1)
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, device), device=device, kv_pages=64, max_batch=4)
+    thread, = _prompts(0, [210], seed=8)
+    n, more = 190, 20
+    keep = torch.ones(1, n, dtype=torch.bool)
+    keep[0, 4:90] = torch.rand(86, generator=torch.Generator().manual_seed(2)) < 0.3
+    gone = (~keep[0]).nonzero()[:, 0]
+    want = _forward_without({k: v.float().cpu() for k, v in sd.items()}, cfg, thread, gone, n)
+    logits = {}
+    for turned in (True, False):
+        pages = [eng.kv.allocator.alloc(pages_for(n))]
+        eng.prefill([thread[:n]], pages)
+        if share:        # another sequence holds the pages: into new ones
+            eng.kv.fork(pages[0], n, [pages_for(n)])
+        pages, (left,) = eng.kv.compact(pages, [n], keep, eng.model.rope if turned else None, room=more + 4)
+        assert left == int(keep.sum())
+        rest = thread[n:]
+        if turned:
+            kept = [t for t, k in zip(thread, keep[0].tolist()) if k]
+            first, out = eng.prefill([kept + rest], pages, return_logits=True, starts=[left])
+            logits[turned] = out[0].float().cpu()
+            steps = [int(first[0])]
+            steps += eng.decode_steps(steps, [left + more], pages, left + more + 4, 3)[0]
+        else:
+            dev = eng.device
+            ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+            table = ints(pages)
+            at = list(range(left, left + more))
+            ws = eng.model.new_workspace(more, 256)
+            out = eng.model.forward(ws, ints(rest), ints(range(n, n + more)), ints([pages[0][a // PAGE] * PAGE + a % PAGE for a in at]),
+                                    table, ints([0] * more), ints([a + 1 for a in at]), more, 256)
+            logits[turned] = out[-1].float().cpu()
+    for got in logits.values():
+        assert float((got - want[-1]).norm() / want[-1].norm()) < 2e-2      # bf16 layers against fp32
+    toks = list(thread)
+    for t in steps:
+        ref = _forward_without({k: v.float().cpu() for k, v in sd.items()}, cfg, toks, gone, n)[-1]
+        assert float(ref.max() - ref[t]) < 2e-2 * float(ref.abs().max())
+        toks.append(t)
 
 
 @pytest.mark.gpu
