@@ -7,7 +7,7 @@ from p2p_llm_chat_go_amd.engine import Engine
 from p2p_llm_chat_go_amd.engine.engine import common_prefix
 from p2p_llm_chat_go_amd.engine.kv_cache import KVCache, PageAllocator, pages_for
 from p2p_llm_chat_go_amd.models import LLAMA31_8B, TINY_LLAMA
-from p2p_llm_chat_go_amd.models.config import rope_table
+from p2p_llm_chat_go_amd.models.config import TINY_LLAMA_GQA, rope_table
 from p2p_llm_chat_go_amd.models.reference import random_state_dict
 from p2p_llm_chat_go_amd.models.weights import EngineWeights
 from tests import prefix_oracle as oracle
@@ -258,6 +258,23 @@ def test_generation_over_a_shared_prefix(device, shared, tails, chunk):
         assert [r.tokens for r in again] == [r.tokens for r in res]
         other = eng.generate(prompts[:1] + prompts, 9, stop_on_eos=False, share_prefix=True)     # another batch of its bucket
         assert [r.tokens for r in other[1:]] == [r.tokens for r in res]
+
+
+@pytest.mark.parametrize("B,shared,own,parts", [(19, 2048, 301, 2), (5, 2048, 301, 2), (5, 32768, 300, 8), (3, 512, 70, 1)])
+def test_decode_graphs_are_planned_for_the_batch_that_they_run(B, shared, own, parts):
+    """Not for the bucket's longest context nor for its rows without a sequence: rows behind a long prefix read it together."""
+    cfg = TINY_LLAMA_GQA.replace(max_pos=40000)
+    sd = random_state_dict(cfg, seed=1)
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, "cpu"), device="cpu", kv_pages=16, max_batch=32)
+    g = eng.shared_decode_graph(B, shared + own, shared // PAGE)
+    plan, _ws = g.state.prefix["prefix"]
+    assert plan.rows == B and shared + own <= plan.max_ctx <= g.state.max_ctx
+    together = [w for w in plan.works.tolist() if w[6] == 0]       # (of 0: pages that a group shares)
+    assert len(together) >= parts and {p for w in together for p in range(w[3], w[4])} == set(range(shared // PAGE))
+    assert eng.shared_decode_graph(B, shared + own - 3, shared // PAGE) is g
+    assert g.state.B > B and bool((g.state.ws.attn == 0).all())     # rows without a sequence attend to nothing
+    plan, _ws = eng.shared_decode_graph(B, shared + own + g.state.max_ctx // 8, shared // PAGE).state.prefix["prefix"]
+    assert plan.max_ctx >= shared + own + g.state.max_ctx // 8      # a longer batch of the same bucket has a plan of its own
 
 
 @pytest.mark.parametrize("device", DEVICES)
