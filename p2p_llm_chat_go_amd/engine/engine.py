@@ -162,6 +162,14 @@ class Engine:
             self._graphs[key] = g
         return g
 
+    def fused_decode(self, B: int, ctx: int) -> bool:
+        """Whether decode steps have projection, rotation and attention in one launch (ops.qkv_attn): up to 256 tokens and 16
+        rows.  They keep it over shared pages too: 2 to 13 sequences behind 64 to 128 tokens, 8 layers, a step is 837 to 1034
+        us so and 855 to 1053 with attention that reads those pages once (at 500 tokens, where it ends, 897 and 874)."""
+        m = self.model
+        return (self.device.type == "cuda" and m.fuse_qkv_attn and isinstance(m.w.layers[0].qkv, torch.Tensor)
+                and ops.qkv_attn_ok(bucket(B, BATCH_BUCKETS), m.nq, m.nkv, bucket(ctx, DECODE_CTX_BUCKETS)))
+
     def shared_decode_graph(self, B: int, ctx: int, pages: int) -> DecodeGraph:
         """The greedy decode graph of B sequences that begin with the same ``pages`` pages (ops.prefix_attention), for
         contexts up to ``ctx``.
@@ -448,7 +456,10 @@ class Engine:
             n_dec = max_new_tokens - 1
             steps_run = 0
             if n_dec > 0 and not all(done):
-                g = self.shared_decode_graph(B, max(need), shared // PAGE) if shared else self.decode_graph(B, max(need))
+                if shared and not self.fused_decode(B, max(need)):
+                    g = self.shared_decode_graph(B, max(need), shared // PAGE)
+                else:
+                    g = self.decode_graph(B, max(need))
                 st = g.state
                 st.load([o[0] for o in out], [len(p) for p in prompts], pages)
                 while steps_run < n_dec:

@@ -260,6 +260,20 @@ def test_generation_over_a_shared_prefix(device, shared, tails, chunk):
         assert [r.tokens for r in other[1:]] == [r.tokens for r in res]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shared,tails,fused", [(130, [5, 1, 30], True), (300, [5, 1, 30], False)])
+def test_steps_of_short_contexts_keep_the_model_s_fused_attention(shared, tails, fused):
+    cfg = TINY_LLAMA
+    sd = random_state_dict(cfg, seed=1)
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, "cuda"), device="cuda", kv_pages=64, max_batch=4)
+    prompts = _prompts(shared, tails)
+    for p, r in zip(prompts, eng.generate(prompts, max_new_tokens=9, stop_on_eos=False, share_prefix=True)):
+        assert len(r.tokens) == 9
+        _greedy_ok(sd, cfg, p, r.tokens)
+    assert bool(eng._graphs) == fused and bool(eng._shared_graphs) != fused
+    assert eng.kv.allocator.free_pages == 63
+
+
 @pytest.mark.parametrize("B,shared,own,parts", [(19, 2048, 301, 2), (5, 2048, 301, 2), (5, 32768, 300, 8), (3, 512, 70, 1)])
 def test_decode_graphs_are_planned_for_the_batch_that_they_run(B, shared, own, parts):
     """Not for the bucket's longest context nor for its rows without a sequence: rows behind a long prefix read it together."""
