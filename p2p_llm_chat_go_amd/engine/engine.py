@@ -119,6 +119,10 @@ class Engine:
         self._prefill_ws = {}
         self._graphs = {}
         self._shared_graphs = {}     # decode graphs of batches that share pages, the last one of every bucket
+        # generate(share_prefix=True) shares from so many tokens on that are not run again: the prompts are two passes over
+        # the weights then.  First tokens, 32 heads on 8, 8 layers: of 2 prompts behind 128 tokens 2.2 ms in one pass and
+        # 2.8 in two, behind 384 3.9 and 3.7, behind 512 4.9 and 3.9; of 5 behind 128 3.4 and 2.9
+        self.share_prefix_min = 512
         # graph-captured prefill chunks (engine.graph.PrefillGraph): dense TP=1 engines on
         # the GPU; P2P_PREFILL_GRAPH=0 keeps every prefill eager
         # TP groups: chunks whose every collective runs on the one-shot IPC kernels (the
@@ -429,13 +433,14 @@ class Engine:
         share_prefix: the tokens that all prompts begin with are run once, and the sequences share
         their full pages of the cache (``KVCache.fork``); attention reads those once for the batch
         (``ops.prefix_attention``).  The numbers are the same up to the order of sums.  Prompts
-        that have less than a page in common run as without it."""
+        that have less than a page in common, or where sharing saves fewer than ``share_prefix_min``
+        tokens, run as without it."""
         t0 = time.perf_counter_ns()
         B = len(prompts)
         assert 0 < B <= self.max_batch
         need = [len(p) + max_new_tokens for p in prompts]
         shared = common_prefix(prompts) if share_prefix and B > 1 else 0
-        if shared < PAGE:
+        if shared < PAGE or shared * (B - 1) < self.share_prefix_min:
             shared = 0
         pages = []
         try:

@@ -260,12 +260,45 @@ def test_generation_over_a_shared_prefix(device, shared, tails, chunk):
         assert [r.tokens for r in other[1:]] == [r.tokens for r in res]
 
 
+@pytest.mark.parametrize("shared,tails,forked", [(600, [5, 1], True), (500, [5, 1], False), (130, [5, 1, 30, 8], False),
+                                                 (260, [5, 1, 30], True), (500, [9], False)])
+def test_prefixes_are_shared_where_that_saves_enough(shared, tails, forked, monkeypatch):
+    cfg = TINY_LLAMA
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(random_state_dict(cfg, seed=1), cfg, "cpu"), device="cpu", kv_pages=64,
+                 max_batch=4)
+    calls, fork = [], eng.kv.fork
+    monkeypatch.setattr(eng.kv, "fork", lambda *a: calls.append(a) or fork(*a))
+    prompts = _prompts(shared, tails)
+    with_it = eng.generate(prompts, 3, stop_on_eos=False, share_prefix=True)
+    assert bool(calls) == forked and eng.kv.allocator.free_pages == 63
+    assert [r.tokens for r in with_it] == [r.tokens for r in eng.generate(prompts, 3, stop_on_eos=False)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shared,tails,chunk", [(100, [5, 1, 30], 1024), (128, [3, 3], 1024), (64, [40, 2], 16), (300, [5, 1, 30], 1024),
+                                                (640, [9, 70, 3], 200)])
+def test_generation_over_every_prefix_of_a_page(device, shared, tails, chunk):
+    """Shared, however little that saves."""
+    cfg = TINY_LLAMA
+    sd = random_state_dict(cfg, seed=1)
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, device), device=device, kv_pages=64, max_prefill_tokens=chunk,
+                 max_batch=4)
+    eng.share_prefix_min = 0
+    prompts = _prompts(shared, tails)
+    for _again in range(2):
+        for p, r in zip(prompts, eng.generate(prompts, max_new_tokens=9, stop_on_eos=False, share_prefix=True)):
+            assert len(r.tokens) == 9 and r.prompt_eval_count == len(p)
+            _greedy_ok(sd, cfg, p, r.tokens)
+    assert eng.kv.allocator.free_pages == 63
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shared,tails,fused", [(130, [5, 1, 30], True), (300, [5, 1, 30], False)])
 def test_steps_of_short_contexts_keep_the_model_s_fused_attention(shared, tails, fused):
     cfg = TINY_LLAMA
     sd = random_state_dict(cfg, seed=1)
     eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, "cuda"), device="cuda", kv_pages=64, max_batch=4)
+    eng.share_prefix_min = 0
     prompts = _prompts(shared, tails)
     for p, r in zip(prompts, eng.generate(prompts, max_new_tokens=9, stop_on_eos=False, share_prefix=True)):
         assert len(r.tokens) == 9
