@@ -537,10 +537,13 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
       float ps = 0.f;
       bf16x8 pf[2];
 #pragma unroll
-      for (int rr = 0; rr < 16; ++rr) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[rr], A.scale_log2, -ms));
-        ps += p;
-        pf[rr >> 3][rr & 7] = f2bf(p);
+      for (int rr = 0; rr < 16; rr += 2) {   // (rounded for the product and summed so, as in a tile)
+        const bf16x2 xy = {f2bf(__builtin_amdgcn_exp2f(fmaf(sc[rr], A.scale_log2, -ms))),
+                           f2bf(__builtin_amdgcn_exp2f(fmaf(sc[rr + 1], A.scale_log2, -ms)))},
+                     ones = {(bf16)1.f, (bf16)1.f};
+        ps = __builtin_amdgcn_fdot2_f32_bf16(xy, ones, ps, false);
+        pf[rr >> 3][rr & 7] = xy[0];
+        pf[rr >> 3][(rr & 7) + 1] = xy[1];
       }
       l = fmaf(l, alpha, ps);
 #pragma unroll

@@ -432,9 +432,10 @@ class Engine:
 
         share_prefix: the tokens that all prompts begin with are run once, and the sequences share
         their full pages of the cache (``KVCache.fork``); attention reads those once for the batch
-        (``ops.prefix_attention``).  The numbers are the same up to the order of sums.  Prompts
-        that have less than a page in common, or where sharing saves fewer than ``share_prefix_min``
-        tokens, run as without it."""
+        (``ops.prefix_attention``).  Its softmax weights are rounded to bf16 before they meet the
+        values (by 2^-8 at most), as they are in prompts; ordinary decode steps keep them in fp32, so
+        that a near tie may fall the other way.  Prompts that have less than a page in common, or where
+        sharing saves fewer than ``share_prefix_min`` tokens, run as without it."""
         t0 = time.perf_counter_ns()
         B = len(prompts)
         assert 0 < B <= self.max_batch

@@ -212,6 +212,21 @@ def test_rows_whose_scores_are_all_minus_infinity_are_nan(way):
     assert bool((got[5] == 0).all())
 
 
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (32, 1)])
+def test_values_that_are_alike_are_the_result(way, Hq, Hkv):
+    """Weights are divided by the sum of the weights as they were multiplied, rounded ones, however many rows share a tile: the
+    mean of equal values is that value but for fp32 sums (300 U32, far below half a step of bf16).  Of every
+    32 keys the others are like one another, so that their weights beside the first's are all rounded by the same."""
+    q, k, v, table, seqs, ctx, rows, most = _batch([(3, 2), (1, 1), (40, 3)], Hq, Hkv, 90, 6)
+    g = torch.Generator().manual_seed(1)
+    alike, first, other = (torch.randn(Hkv, 1, D, generator=g).bfloat16() for _ in range(3))
+    k = torch.where(torch.isnan(k), k, torch.where((torch.arange(PAGE) % 32 == 0)[:, None], first, other))
+    v = torch.where(torch.isnan(v), v, alike)
+    plan = ops.prefix_plan(rows, Hq, Hkv, most, DEV)
+    got = _run(q, k, v, table, ctx, plan).cpu().view(-1, Hkv, Hq // Hkv, D)
+    assert torch.equal(got, alike[None].expand_as(got))
+
+
 def test_values_near_the_type_s_largest(way):
     """Weights sum to 1: a result is no larger than its values, whatever the sums before the division are."""
     q, k, v, table, seqs, ctx, rows, most = _batch([(12, 2), (6, 1)], 8, 2, 90, 5)
