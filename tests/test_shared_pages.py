@@ -415,6 +415,19 @@ def test_a_sequence_goes_on_behind_a_compaction(device, share):
         toks.append(t)
 
 
+def test_prompts_whose_tables_do_not_share_their_pages_are_refused():
+    cfg = TINY_LLAMA
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(random_state_dict(cfg, seed=2), cfg, "cpu"), device="cpu", kv_pages=64)
+    prompts = _prompts(150, [7, 80])
+    pages = [eng.kv.allocator.alloc(4)]
+    eng.prefill([prompts[0][:150]], pages)
+    pages += eng.kv.fork(pages[0], 150, [4])
+    eng.prefill(prompts, pages, starts=[150] * 2, shared_pages=2)
+    for tables, n in (([pages[0], [pages[1][0]] + pages[1][2:]], 2), (pages, 3), ([pages[0], pages[1][:1]], 2), (pages, -1)):
+        with pytest.raises(ValueError, match="share"):
+            eng.prefill(prompts, tables, starts=[200] * 2, shared_pages=n)
+
+
 @pytest.mark.gpu
 def test_forks_attention_and_compaction_one_after_the_other():
     """A thread forks, rows of both attend the shared pages, tokens leave both, and rows attend what is left."""
