@@ -30,6 +30,9 @@ def _caches(k: torch.Tensor, v: torch.Tensor, what: str):
     if k1 != 1 or v1 != 1 or kt != HEAD_DIM or vt != HEAD_DIM or (kl | kp | kh | vl | vp | vh) * size % 16 or (ka | va) % 16:
         raise ValueError("%s: the tokens of a page must be contiguous and start at multiples of 16 bytes" % what)
     layers, pages, heads = shape[:3]
+    if not (kl and kp and kh and vl and vp and vh) and any(n > 1 and not (a and b)
+                                                           for n, a, b in ((layers, kl, vl), (pages, kp, vp), (heads, kh, vh))):
+        raise ValueError("%s: layers, pages and heads must have memory of their own" % what)
     return (ka, va, _SIX(kl * size, kp * size, kh * size, vl * size, vp * size, vh * size), layers, heads, pages,
             HEAD_DIM * size), dev
 

@@ -172,6 +172,21 @@ def test_caches_that_are_refused(k, v):
         ops.compact_pages(k, k if v is None else v, torch.ones(1, 1, **i32), torch.ones(1, **i32), torch.ones(1, 3, dtype=torch.bool))
 
 
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_caches_that_repeat_their_memory_are_refused(dim):
+    """An expanded cache has one memory for several layers, pages or heads, which would be written at once."""
+    k, v = _pages()
+    again = k.select(dim, 0).unsqueeze(dim).expand_as(k)
+    i32 = dict(dtype=torch.int32)
+    for a, b in ((again, v), (v, again)):
+        with pytest.raises(ValueError, match="memory of their own"):
+            ops.copy_pages(a, b, [1], [2])
+        with pytest.raises(ValueError, match="memory of their own"):
+            ops.compact_pages(a, b, torch.ones(1, 1, **i32), torch.ones(1, **i32), torch.ones(1, 3, dtype=torch.bool))
+    one = k[:1, :, :1]
+    ops.copy_pages(one.expand(1, -1, 1, -1, -1), one.clone(), [1], [2])
+
+
 def test_nothing_to_copy():
     k, v = _pages()
     k[:, 3] = 1
