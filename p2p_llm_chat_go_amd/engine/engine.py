@@ -123,6 +123,10 @@ class Engine:
         # the weights then.  First tokens, 32 heads on 8, 8 layers: of 2 prompts behind 128 tokens 2.2 ms in one pass and
         # 2.8 in two, behind 384 3.9 and 3.7, behind 512 4.9 and 3.9; of 5 behind 128 3.4 and 2.9
         self.share_prefix_min = 512
+        # ... and its steps read shared pages once from so many bytes of a layer's K and V on that they do not read again:
+        # a graph of another batch or number of shared pages is captured first, about 1 ms a layer, as long as those bytes
+        # take at 5 TB/s (64 steps of 2 sequences behind 512 tokens 69.0 ms with the capture where ordinary steps have 63.3)
+        self.share_steps_min = 5 * 10 ** 9
         # graph-captured prefill chunks (engine.graph.PrefillGraph): dense TP=1 engines on
         # the GPU; P2P_PREFILL_GRAPH=0 keeps every prefill eager
         # TP groups: chunks whose every collective runs on the one-shot IPC kernels (the
@@ -182,17 +186,32 @@ class Engine:
         context and all of its rows, 5 sequences behind 8192 tokens read those one by one (32 heads on 8, 8 layers: a step
         1044 us, 991 so; 19 behind 2048 1618 and 1586).  The bucket's other rows are behind the plan's: attention leaves
         theirs at the workspace's zeros."""
-        key = (bucket(B, BATCH_BUCKETS), bucket(ctx, CTX_BUCKETS))
-        step = max(PAGE, key[1] // 16)
-        longest = -(-ctx // step) * step
+        key, batch = self._shared_batch(B, ctx, pages)
         have = self._shared_graphs.get(key)
-        if have is None or have[0] != (B, pages, longest):
+        if have is None or have[0] != batch:
             self._shared_graphs.pop(key, None)
             st = DecodeState(self.model, key[0], key[1] // PAGE, key[1], key[1])
-            plan = ops.prefix_plan([(B, pages)], self.model.nq, self.model.nkv, longest, self.device)
+            plan = ops.prefix_plan([(B, pages)], self.model.nq, self.model.nkv, batch[2], self.device)
             st.prefix = {"prefix": (plan, ops.prefix_workspace(plan))}
-            have = self._shared_graphs[key] = ((B, pages, longest), DecodeGraph(st, self.use_graph).capture())
+            have = self._shared_graphs[key] = (batch, DecodeGraph(st, self.use_graph).capture())
         return have[1]
+
+    def _shared_batch(self, B: int, ctx: int, pages: int):
+        """(bucket, what a graph of it is for) of shared_decode_graph."""
+        key = (bucket(B, BATCH_BUCKETS), bucket(ctx, CTX_BUCKETS))
+        step = max(PAGE, key[1] // 16)
+        return key, (B, pages, -(-ctx // step) * step)
+
+    def shared_steps(self, B: int, ctx: int, pages: int, steps: int) -> bool:
+        """Whether so many decode steps of B sequences are worth a graph that reads their first pages once: it is there, or
+        the K and V bytes of a layer that the steps do not read again are ``share_steps_min``."""
+        if self.fused_decode(B, ctx):
+            return False
+        key, batch = self._shared_batch(B, ctx, pages)
+        have = self._shared_graphs.get(key)
+        if (have is not None and have[0] == batch) or not (self.use_graph and self.device.type == "cuda"):
+            return True
+        return steps * (B - 1) * pages * self.kv.bytes_per_page(self.cfg, self.model.tp) >= self.share_steps_min * self.cfg.n_layers
 
     def prefill_graph_key(self, rows: int, n_seq: int, max_ctx: int, greedy: bool = True):
         return (bucket(rows, PREFILL_ROW_BUCKETS), min(bucket(n_seq, BATCH_BUCKETS), self.max_batch),
@@ -438,7 +457,8 @@ class Engine:
         (``ops.prefix_attention``).  Its softmax weights are rounded to bf16 before they meet the
         values (by 2^-8 at most), as they are in prompts; ordinary decode steps keep them in fp32, so
         that a near tie may fall the other way.  Prompts that have less than a page in common, or where
-        sharing saves fewer than ``share_prefix_min`` tokens, run as without it."""
+        sharing saves fewer than ``share_prefix_min`` tokens, run as without it; decode steps read shared
+        pages together where that earns its graph (``shared_steps``)."""
         t0 = time.perf_counter_ns()
         B = len(prompts)
         assert 0 < B <= self.max_batch
@@ -465,7 +485,7 @@ class Engine:
             n_dec = max_new_tokens - 1
             steps_run = 0
             if n_dec > 0 and not all(done):
-                if shared and not self.fused_decode(B, max(need)):
+                if shared and self.shared_steps(B, max(need), shared // PAGE, n_dec):
                     g = self.shared_decode_graph(B, max(need), shared // PAGE)
                 else:
                     g = self.decode_graph(B, max(need))

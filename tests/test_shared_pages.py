@@ -283,7 +283,7 @@ def test_generation_over_every_prefix_of_a_page(device, shared, tails, chunk):
     sd = random_state_dict(cfg, seed=1)
     eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, device), device=device, kv_pages=64, max_prefill_tokens=chunk,
                  max_batch=4)
-    eng.share_prefix_min = 0
+    eng.share_prefix_min = eng.share_steps_min = 0
     prompts = _prompts(shared, tails)
     for _again in range(2):
         for p, r in zip(prompts, eng.generate(prompts, max_new_tokens=9, stop_on_eos=False, share_prefix=True)):
@@ -298,12 +298,29 @@ def test_steps_of_short_contexts_keep_the_model_s_fused_attention(shared, tails,
     cfg = TINY_LLAMA
     sd = random_state_dict(cfg, seed=1)
     eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, "cuda"), device="cuda", kv_pages=64, max_batch=4)
-    eng.share_prefix_min = 0
+    eng.share_prefix_min = eng.share_steps_min = 0
     prompts = _prompts(shared, tails)
     for p, r in zip(prompts, eng.generate(prompts, max_new_tokens=9, stop_on_eos=False, share_prefix=True)):
         assert len(r.tokens) == 9
         _greedy_ok(sd, cfg, p, r.tokens)
     assert bool(eng._graphs) == fused and bool(eng._shared_graphs) != fused
+    assert eng.kv.allocator.free_pages == 63
+
+
+@pytest.mark.gpu
+def test_a_graph_over_shared_pages_is_captured_where_its_steps_earn_it():
+    cfg = TINY_LLAMA
+    sd = random_state_dict(cfg, seed=1)
+    eng = Engine(cfg, weights=EngineWeights.from_state_dict(sd, cfg, "cuda"), device="cuda", kv_pages=64, max_batch=4)
+    # a page of a layer's K and V are 32 KB: 8 steps of 2 more sequences behind 10 pages do not read 5.2 MB again
+    prompts = _prompts(650, [5, 1, 30])
+    for least, captured in ((8 * 2 * 10 * 32768 + 1, False), (8 * 2 * 10 * 32768, True), (10 ** 9, True)):
+        eng.share_steps_min = least
+        for p, r in zip(prompts, eng.generate(prompts, max_new_tokens=9, stop_on_eos=False, share_prefix=True)):
+            assert len(r.tokens) == 9
+            _greedy_ok(sd, cfg, p, r.tokens)
+        assert bool(eng._shared_graphs) == captured       # (and one that is there is taken, whatever the steps)
+    assert not eng.shared_steps(3, 690, 9, 8) and eng.shared_steps(3, 690, 10, 1)
     assert eng.kv.allocator.free_pages == 63
 
 
