@@ -98,9 +98,9 @@ __device__ __forceinline__ int set_of_8(const uint8_t* p) {
 
 // Into other pages: a workgroup takes 256 / TPT consecutive places of one sequence, counts the kept ones before them, and
 // moves them in the layers and heads of its share (blockIdx.z): the turn's numbers are formed once for all of them.  Places that
-// are not kept are not read.  Bound by memory: 7 sequences of 2301 places in 8 layers, half of them kept, 616 MB in 133 us = 4.6
-// TB/s, 6 of 8150 turned 1881 MB in 390 us = 4.8; 1000 places in 32 layers, 170 MB in 41 us, where one round of workgroups has
-// its chain of counting, page numbers, angles, rows and stores.
+// are not kept are not read.  Bound by memory (8 heads, half of the tokens kept): 6 sequences of 8150 places in 8 layers, 0.8 GB
+// read and as much written, 331 us = 4.8 TB/s, turned 332; one of 1000 in 32 layers, 131 MB, 30 and 31 us, where one round of
+// workgroups has its chain of counting, page numbers, angles, rows and stores.
 template <int TPT, bool TURN>
 __global__ __launch_bounds__(256) void compact_apart_kernel(Cache k, Cache v, Sequences s, int heads, int layers,
                                                             const float* __restrict__ cos_sin) {
@@ -151,8 +151,9 @@ __global__ __launch_bounds__(256) void compact_apart_kernel(Cache k, Cache v, Se
 // In place: one workgroup moves all of a sequence's tokens of HEADS heads, a round of 1024 / TPT places after the other.  A place
 // n takes the token of a place p >= n: once the workgroup has read a round's places no later read meets what it writes, and the
 // next round's reads go out before this one's writes.  1024 threads, since what a CU has in flight is one round: 6 sequences of
-// 8150 places in 8 layers, 0.8 GB read and as much written, 352 us = 4.5 TB/s, turned 450; with few sequences it is bound by
-// the chain of rounds, some 2.2 us each (1000 places in 8 layers 20 us, turned 31, into other pages 9 and 11).  Reading `keep`
+// 8150 places in 8 layers (8 heads, half kept), 0.8 GB read and as much written, 356 us = 4.5 TB/s, turned 453; with few
+// sequences it is bound by the chain of rounds, some 2.2 us each (one of 1000 in 8 layers 21 us, turned 32, into other pages
+// 10 and 11).  Reading `keep`
 // two rounds ahead and unrolled rounds gave nothing.
 template <int TPT, bool TURN, int HEADS>
 __global__ __launch_bounds__(1024) void compact_inside_kernel(Cache k, Cache v, Sequences s, int heads,
@@ -250,8 +251,9 @@ __global__ __launch_bounds__(1024) void compact_inside_kernel(Cache k, Cache v, 
 template <int TPT, bool TURN>
 int compact(Cache k, Cache v, const Sequences& s, int n, int heads, int layers, const float* cos_sin, hipStream_t st) {
   if (!s.to) {
-    // Two heads in flight per workgroup, once that leaves 192 workgroups: six sequences of 8150 places in 8 layers turned
-    // 613 -> 450 us, as they are 416 -> 352, six of 1000 66 -> 48 and 45 -> 39; three of 1000 would lose, 36 -> 41 and 25 -> 30.
+    // Two heads in flight per workgroup, once that leaves 192 workgroups (8 heads, half of the tokens kept): six sequences of
+    // 8150 places in 8 layers turned 616 -> 453 us, as they are 421 -> 356, six of 1000 75 -> 56 and 57 -> 49, two of 1000 in 32
+    // layers 82 -> 64 and 65 -> 56; three of 1000 in 8 would lose, 36 -> 41 and 26 -> 30, one in 32 40 -> 46 and 31 -> 37.
     if (heads % 2 == 0 && heads * layers * n >= 384)
       hipLaunchKernelGGL((compact_inside_kernel<TPT, TURN, 2>), dim3(heads / 2 * layers, n), dim3(1024), 0, st, k, v, s, heads, cos_sin);
     else
@@ -261,7 +263,7 @@ int compact(Cache k, Cache v, const Sequences& s, int n, int heads, int layers, 
   constexpr int TOK = 256 / TPT;
   const int chunks = max(1, (min(s.places, s.width * PAGE) + TOK - 1) / TOK), all = heads * layers;
   // Eight (layer, head) pairs for a workgroup, which counts kept places and forms angles once for them: six sequences of 8150
-  // places in 8 layers turned 331 us, with one pair each 448, with all 64 349 (as they are 328, 338, 347).  Fewer where
+  // places in 8 layers of 8 heads, half kept, turned 332 us, with one pair each 448, with all 64 349 (as they are 331, 338, 347).  Fewer where
   // there would not be 256 workgroups: one layer of 1000 places 7.6 -> 6.3.
   const int shares = max(max(1, all / 8), min(all, 256 / max(1, chunks * n)));
   hipLaunchKernelGGL((compact_apart_kernel<TPT, TURN>), dim3(chunks, n, shares), dim3(256), 0, st, k, v, s, heads, layers, cos_sin);

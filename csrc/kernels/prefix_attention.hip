@@ -10,7 +10,7 @@
 //
 // What it takes, calls one after the other: 2 rows behind 256 tokens 7 us (the host 8), 19 behind 2048 13 and 41 on one kv head
 // 15, of which the second launch is 3: chains of loads of some 0.7 us each (work, page numbers, keys, values) and the launches.
-// 704 prompt rows behind 1536 tokens 34 us, 64 rows of 64 heads behind 32768 107 us: the products, see the tiles.
+// 704 prompt rows behind 1536 tokens 34 us, 64 rows of 64 heads behind 32768 108 us: chains between the products, see the tiles.
 #include "common.h"
 #include "lds_pipe.h"
 
@@ -201,12 +201,14 @@ __device__ __forceinline__ bf16x8 read_v8(const bf16* p) {
 // scores, maxima, sums and O are fp32.
 //
 // A wavefront reads a page's K and V from LDS, 32 KB, for 32 matrix instructions of 32 cycles: two workgroups on a CU have 2050
-// cycles of either for a page each, and take 2980 (one alone 2480 for 1024 of each).  The rest is the maxima, on which the
-// exponentials wait, and the wait for copies at a page's start.  64 rows of 64 heads behind 32768 tokens: 70 GFLOP in 100 us.
+// cycles of either for a page each, and take 4300 to 4900 (2.0 to 2.3 us at 2.13 GHz, the clock under this load), also where
+// all pages are one that the caches hold: a wavefront's chain of maxima, exponentials and waits at a page's start, which one
+// other wavefront on its SIMD does not cover.  64 rows of 64 heads behind 32768 tokens, 69 GFLOP: 81 us, of which launch, first
+// loads and 34 MB of results 12.
 // Three stages of K, a barrier of its own for V, copies spread between the products, LDS reads three pairs ahead and both
 // products interleaved (which spills) gave nothing.
 // 128 pairs, since a wavefront's registers hold 32 (O 64, Q 64, S and P 64) and four are a CU's quarters: with 32 pairs for a
-// workgroup 241 us, 129 then with 128.
+// workgroup 241 us, 129 then with 128 (with the rows' own tokens and the second launch).
 template <int KG>
 __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh, bf16* lds_all, float2* sml, int wave, int lane) {
   constexpr int CW = 4, CP = 16 / CW;                       // wavefronts that copy a page together, copies of each

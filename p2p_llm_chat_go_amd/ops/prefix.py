@@ -285,7 +285,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     Row r attends the first ``min(ctx_lens[r], plan.max_ctx)`` tokens of its block table; a row that sees none is 0.  Rows
     behind the plan's are not read or written; out is other memory than q.  A group's shared pages are read through its
-    first row's table.  Block tables hold pages of the cache; others read page 0 or the last one.  scale: 2^-64 .. 2^64 (None: 128^-0.5)."""
+    first row's table.  Block tables hold pages of the cache; others read page 0 or the last one.  scale: 2^-64 .. 2^64
+    (None: 128^-0.5).  Scores, softmax statistics and sums are fp32; weights are rounded to bf16 (by 2^-8 at most) for the
+    product with the values, and divided by the sum of the rounded ones."""
     R, n_heads, n_kv = plan.rows, plan.n_heads, plan.n_kv
     width = n_heads * HEAD_DIM
     if scale is None:
