@@ -306,7 +306,7 @@ class Engine:
         """
         if shared_pages and (pad_rows is not None or any(s0 < shared_pages * PAGE for s0 in starts or [0])):
             raise ValueError("prefill: shared pages hold tokens before every start, without dummy rows")
-        if shared_pages and (shared_pages < 0 or any(len(t) < shared_pages or t[:shared_pages] != block_tables[0][:shared_pages]
+        if shared_pages and (shared_pages < 0 or any(len(t) < shared_pages or list(t[:shared_pages]) != list(block_tables[0][:shared_pages])
                                                      for t in block_tables)):
             raise ValueError("prefill: the block tables do not share their first %d pages" % shared_pages)
         sampled = sampling is not None and not all(p.greedy for p in sampling)

@@ -440,6 +440,7 @@ def test_prompts_whose_tables_do_not_share_their_pages_are_refused():
     eng.prefill([prompts[0][:150]], pages)
     pages += eng.kv.fork(pages[0], 150, [4])
     eng.prefill(prompts, pages, starts=[150] * 2, shared_pages=2)
+    eng.prefill(prompts, [tuple(pages[0]), torch.tensor(pages[1])], starts=[150] * 2, shared_pages=2)    # whatever holds the numbers
     for tables, n in (([pages[0], [pages[1][0]] + pages[1][2:]], 2), (pages, 3), ([pages[0], pages[1][:1]], 2), (pages, -1)):
         with pytest.raises(ValueError, match="share"):
             eng.prefill(prompts, tables, starts=[200] * 2, shared_pages=n)
