@@ -161,10 +161,10 @@ __device__ void exact_pair(const Args& A, const int* btr, int r, int h, int lane
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
 // A pair's result from its only part: lane r32 has numbers 4 r32 ..  True: it has to be done again.
-__device__ __forceinline__ bool put_result(const Args& A, long at, f32x4 sum, float den, int r32) {
+__device__ __forceinline__ bool put_result(const Args& A, long at, f32x4 sum, float den, bool sees, int r32) {
   const float by = 1.f / den;
   bf16x4 y;
-  bool bad = den == 0.f;   // (no key, or none of a score above -inf)
+  bool bad = den == 0.f && sees;   // (no score above -inf)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float x = den == 0.f ? 0.f : sum[i] * by;   // (whatever the values of others are)
@@ -412,6 +412,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
   if (!whole && (KG == 1 || S.first >= S.end) && kg == 0 && hh == 0 && to >= 0) A.part_ml[to / HD] = make_float2(m, l);
   if (!whole && S.first >= S.end) return;   // a part of no page has its maximum only
   // the wavefront's rows to LDS and from there in whole rows, of both page groups: 32 / KG pairs for a wavefront
+  const unsigned sees = (unsigned)__ballot(lim > 0);   // pairs that see a key
   float* so = reinterpret_cast<float*>(lds_all);
   put_rows(so + wave * (32 * HD), o, r32, hh);
   if constexpr (KG > 1) {
@@ -437,7 +438,7 @@ __device__ __forceinline__ void tile_role(const Args& A, const Work& W, int kvh,
       if (!whole && at >= 0 && r32 == 0) A.part_ml[at / HD] = make_float2(M, den);
     }
     if (at < 0) continue;
-    if (whole) bad |= (unsigned)put_result(A, at, sum, den, r32) << i;
+    if (whole) bad |= (unsigned)put_result(A, at, sum, den, sees >> p & 1, r32) << i;
     else *reinterpret_cast<f32x4*>(A.part_o + at + 4 * r32) = sum;
   }
   if (__builtin_expect(__any(bad), 0)) {
@@ -582,6 +583,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
   if (hh == 0) sml[w * ROWS + r32] = make_float2(m == -INFINITY ? m : m * A.scale_log2, l);
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(lds_all);
+  const unsigned sees = (unsigned)__ballot(lim > 0);   // pairs that see a key
   unsigned bad = 0;
 #pragma unroll
   for (int i = 0; i < ROWS * 32 / (NW * 64); ++i) {
@@ -603,7 +605,7 @@ __device__ __forceinline__ void few_role(const Args& A, const Work& W, int kvh, 
     }
     if (at < 0) continue;
     if (whole) {
-      bad |= (unsigned)put_result(A, at, sum, den, r32) << i;
+      bad |= (unsigned)put_result(A, at, sum, den, sees >> p & 1, r32) << i;
       continue;
     }
     *reinterpret_cast<f32x4*>(A.part_o + at + 4 * r32) = sum;
